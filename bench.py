@@ -36,22 +36,25 @@ FP32_VECTOR_PEAK_TFLOPS = 157.3  # MI355X published fp32 vector (packed-FMA) pea
 # belong to the kernels being timed, and the fields derived from them are reported as null.
 C1_PROFILE = {
     "source": "profiles/k_fwd_sep_k_bwd_sep_c1_B16_N8192_256x256_C3.md",
-    "csrc_sha16": "a244c3e3a6718d95",
+    "csrc_sha16": "b10d8cf631def163",
     "bwd": {"fma": 6.862e8, "mul": 7.632e7, "add": 7.615e7, "trans": 6.770e7, "fetch_kib": 55720, "write_kib": 147400},
     "fwd": {"fma": 1.386e8, "mul": 1.269e7, "add": 8.919e6, "trans": 6.714e7, "mfma": 6.707e7, "fetch_kib": 12700, "write_kib": 131100},
 }
 
 
 def csrc_sha16():
-    """First 16 hex digits of the SHA-256 over the kernel sources (igs_amd/csrc/*, include/igs_hip.h), in name order."""
+    """First 16 hex digits of the SHA-256 over the sources of the splat's kernels, in name order: the translation
+    unit igs_gs2d.hip, the files it includes and include/igs_hip.h (other units of the library are not among them)."""
     import hashlib
+    import re
 
     h = hashlib.sha256()
     csrc = os.path.join(ROOT, "igs_amd", "csrc")
-    for path in sorted(os.path.join(csrc, f) for f in os.listdir(csrc)) + [os.path.join(ROOT, "include", "igs_hip.h")]:
-        if os.path.isfile(path):
-            h.update(os.path.basename(path).encode())
-            h.update(open(path, "rb").read())
+    unit = os.path.join(csrc, "igs_gs2d.hip")
+    names = re.findall(r'^#include "(igs_\w+\.h)"', open(unit).read(), flags=re.M)
+    for path in sorted([unit] + [os.path.join(csrc, n) for n in names if n != "igs_hip.h"]) + [os.path.join(ROOT, "include", "igs_hip.h")]:
+        h.update(os.path.basename(path).encode())
+        h.update(open(path, "rb").read())
     return h.hexdigest()[:16]
 
 

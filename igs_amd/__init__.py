@@ -16,6 +16,15 @@ from .gs2d import (  # noqa: F401
 )
 
 from ._splat import exact, library_options  # noqa: F401,E402
+from .feature import (  # noqa: F401,E402
+    dropout,
+    dropout_keep_mask,
+    embedding_lookup,
+    layer_norm,
+    naive_dropout,
+    naive_embedding_lookup,
+    naive_layer_norm,
+)
 from .fit import GaussianImageFit  # noqa: F401,E402
 from .reg import koleo_diversity_loss  # noqa: F401,E402
 
@@ -24,6 +33,13 @@ __all__ = [
     "library_options",
     "GaussianImageFit",
     "koleo_diversity_loss",
+    "embedding_lookup",
+    "layer_norm",
+    "dropout",
+    "dropout_keep_mask",
+    "naive_embedding_lookup",
+    "naive_layer_norm",
+    "naive_dropout",
     "GaussianSplatting2D",
     "gaussian_splatting_2d",
     "naive_gaussian_2d",

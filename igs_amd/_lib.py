@@ -14,7 +14,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 LIB_PATH = os.environ.get("IGS_HIP_LIBRARY") or os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                                                "libigs_hip.so")
 
-ABI_VERSION = 8  # IGS_ABI_VERSION of include/igs_hip.h this binding was written against
+ABI_VERSION = 9  # IGS_ABI_VERSION of include/igs_hip.h this binding was written against
 IGS_GRID_GENERAL = 0
 IGS_GRID_SEPARABLE = 1
 IGS_GRID_AUTO = 2
@@ -22,6 +22,7 @@ IGS_OPT_NO_CULL = 0x100
 IGS_OPT_BIN_LEVELS_1 = 0x200
 IGS_OPT_BIN_LEVELS_2 = 0x400
 IGS_OPT_LISTS_BUILT = 0x800
+IGS_F32, IGS_F16, IGS_BF16 = 0, 1, 2   # igs_dtype
 IGS_MAX_CHANNELS = 16
 IGS_STATIC_SCRATCH_BYTES = 64 << 20
 COMPILED_CHANNELS = (1, 2, 3, 4, 8, 16)
@@ -67,6 +68,18 @@ class KoleoPlan(ctypes.Structure):
         ("saved_bytes", c_uint64),
         ("scratch_bytes", c_uint64),
     ]
+
+
+class EmbeddingPlan(ctypes.Structure):
+    """Mirror of igs_embedding_plan_t."""
+
+    _fields_ = [("vocab", c_int64), ("count", c_int64), ("D", c_int32), ("reserved", c_int32), ("ws_bytes", c_uint64)]
+
+
+class LayerNormPlan(ctypes.Structure):
+    """Mirror of igs_layer_norm_plan_t."""
+
+    _fields_ = [("rows", c_int64), ("D", c_int32), ("partials", c_int32), ("ws_bytes", c_uint64)]
 
 
 _FP = c_void_p  # device pointers travel as plain addresses
@@ -118,6 +131,16 @@ SIGNATURES = {
     "igs_koleo_plan": (c_int, [c_int, c_int, c_int, POINTER(KoleoPlan)]),
     "igs_koleo_forward": (c_int, [_FP, c_int, c_int, c_int, _FP, _FP, c_size_t, _FP, c_size_t, c_void_p]),
     "igs_koleo_backward": (c_int, [_FP, c_size_t, _FP, c_int, c_int, c_int, _FP, c_void_p]),
+    "igs_embedding_forward": (c_int, [_FP, c_int64, c_int, c_int64, c_int, _FP, c_int, c_int64, c_float, _FP, c_void_p]),
+    "igs_embedding_plan": (c_int, [c_int64, c_int, c_int, c_int64, POINTER(EmbeddingPlan)]),
+    "igs_embedding_backward": (c_int, [_FP, c_int, _FP, c_int, c_int64, c_int64, c_int, c_float, c_int64, _FP, c_void_p,
+                                       c_size_t, c_void_p]),
+    "igs_dropout": (c_int, [_FP, c_int, c_int64, c_int, c_uint64, _FP, c_uint64, _FP, c_void_p]),
+    "igs_layer_norm_forward": (c_int, [_FP, c_int64, c_int, _FP, _FP, c_int, c_int64, c_int, c_float, c_int, c_uint64,
+                                       _FP, c_uint64, _FP, _FP, c_void_p]),
+    "igs_layer_norm_plan": (c_int, [c_int64, c_int, c_int, c_int, POINTER(LayerNormPlan)]),
+    "igs_layer_norm_backward": (c_int, [_FP, _FP, c_int64, c_int, _FP, c_int, _FP, c_int64, c_int, c_int, c_uint64, _FP,
+                                        c_uint64, _FP, _FP, _FP, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None
@@ -172,6 +195,22 @@ def koleo_plan(B: int, N: int, D: int) -> KoleoPlan:
     p = KoleoPlan()
     check(load().igs_koleo_plan(B, N, D, ctypes.byref(p)), "igs_koleo_plan")
     return p
+
+
+@functools.lru_cache(maxsize=256)
+def embedding_workspace_bytes(vocab: int, D: int, dtype: int, count: int) -> int:
+    """Scratch of the lookup's dense gradient (pure host arithmetic in the library; cached)."""
+    p = EmbeddingPlan()
+    check(load().igs_embedding_plan(vocab, D, dtype, count, ctypes.byref(p)), "igs_embedding_plan")
+    return p.ws_bytes
+
+
+@functools.lru_cache(maxsize=256)
+def layer_norm_workspace_bytes(rows: int, D: int, dtype: int, wdtype: int) -> int:
+    """Scratch of the norm's backward (pure host arithmetic in the library; cached)."""
+    p = LayerNormPlan()
+    check(load().igs_layer_norm_plan(rows, D, dtype, wdtype, ctypes.byref(p)), "igs_layer_norm_plan")
+    return p.ws_bytes
 
 
 def strides6(sx, sy):

@@ -11,7 +11,7 @@ import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
-SOURCES = [os.path.join(PKG, "csrc", "igs_gs2d.hip")]
+SOURCES = [os.path.join(PKG, "csrc", f) for f in ("igs_gs2d.hip", "igs_feature.hip")]
 LIB = os.path.join(PKG, "libigs_hip.so")
 
 # Packed-fp32 instruction selection is switched off for all device code.

@@ -1,0 +1,239 @@
+// igs_feature.hip -- the operators in front of the module's head (the features that
+// src/igs/gs2d.py:611-635 of the reference takes as given): embedding lookup with its dense gradient,
+// layer norm forward and backward, dropout from a counter-based generator.  Kernels in the included
+// headers, argument checks and launches here.
+//
+// All of them are bound by memory traffic (a few operations per element); the sums of gradients over
+// rows or repeated tokens have a fixed order, so results are bit-reproducible run to run.
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include "igs_hip.h"
+
+namespace {
+#include "igs_feature_common.h"
+
+#include "igs_dropout.h"
+#include "igs_embedding.h"
+#include "igs_layer_norm.h"
+
+constexpr int64_t kMaxCount = 0x7FFFFFFE;
+constexpr int kMaxRow = 1 << 20;
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t at_most(int64_t v, int64_t most) { return v < most ? v : most; }
+
+inline int launch_status() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? IGS_OK : (int)e;
+}
+
+inline bool dtype_ok(int t) { return t == IGS_F32 || t == IGS_F16 || t == IGS_BF16; }
+inline int dtype_bytes(int t) { return t == IGS_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+int make_dropout(int threshold, uint64_t seed, const uint64_t* seed_device, uint64_t offset, Dropout* d) {
+    if (threshold < 0 || threshold > 65536) return IGS_ERR_BAD_ARGUMENT;
+    if (!aligned_to(seed_device, 8)) return IGS_ERR_ALIGNMENT;
+    d->threshold = (uint32_t)threshold;
+    d->factor = threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.0f;
+    d->seed = seed;
+    d->offset = offset;
+    d->seed_device = seed_device;
+    return IGS_OK;
+}
+
+int embedding_shape(int64_t vocab, int D, int64_t count) {
+    if (vocab < 1 || vocab > kMaxCount || D < 1 || D > kMaxRow || count < 0 || count > kMaxCount) return IGS_ERR_BAD_SHAPE;
+    return IGS_OK;
+}
+
+int embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding_plan_t* p) {
+    if (!p) return IGS_ERR_NULL_POINTER;
+    if (!dtype_ok(dtype)) return IGS_ERR_BAD_DTYPE;
+    const int rc = embedding_shape(vocab, D, count);
+    if (rc) return rc;
+    p->vocab = vocab;
+    p->count = count;
+    p->D = D;
+    p->reserved = 0;
+    p->ws_bytes = 0;
+    return IGS_OK;
+}
+
+int norm_shape(int64_t rows, int D, int dtype, int wdtype) {
+    if (!dtype_ok(dtype) || (wdtype != dtype && wdtype != IGS_F32)) return IGS_ERR_BAD_DTYPE;
+    if (rows < 0 || rows > kMaxCount || D < 1 || D > kMaxRow) return IGS_ERR_BAD_SHAPE;
+    return IGS_OK;
+}
+
+int norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* p) {
+    if (!p) return IGS_ERR_NULL_POINTER;
+    const int rc = norm_shape(rows, D, dtype, wdtype);
+    if (rc) return rc;
+    p->rows = rows;
+    p->D = D;
+    p->partials = 0;
+    p->ws_bytes = 0;
+    return IGS_OK;
+}
+
+template <class T, class I>
+int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, const void* tokens, int64_t count,
+                     float scale, void* out, hipStream_t st) {
+    const int64_t blocks = at_most(ceil_div(count * D, kBlock), 1 << 20);
+    hipLaunchKernelGGL((k_embed_fwd<T, I>), dim3(blocks), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
+                       (const I*)tokens, count, scale, (T*)out);
+    return launch_status();
+}
+
+template <class T, class I>
+int launch_embed_bwd(const void* grad, const void* tokens, int64_t count, int64_t vocab, int D, float scale,
+                     int64_t padding, void* out, hipStream_t st) {
+    hipLaunchKernelGGL((k_embed_bwd<T, I>), dim3(at_most(vocab, 1 << 20)), dim3(kBlock), 0, st, (const T*)grad,
+                       (const I*)tokens, count, vocab, D, scale, padding, (T*)out);
+    return launch_status();
+}
+
+template <class T>
+int launch_dropout(const void* x, int64_t count, const Dropout& d, void* y, hipStream_t st) {
+    const int64_t blocks = at_most(ceil_div(ceil_div(count, 8), kBlock), 1 << 20);
+    hipLaunchKernelGGL((k_dropout<T>), dim3(blocks), dim3(kBlock), 0, st, (const T*)x, count, d, (T*)y);
+    return launch_status();
+}
+
+template <class T, class W>
+int launch_norm_fwd(const void* x, int64_t stride, const void* w, const void* b, int64_t rows, int D, float eps,
+                    const Dropout& d, void* y, float* stats, hipStream_t st) {
+    hipLaunchKernelGGL((k_norm_fwd<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kBlock), 0, st, (const T*)x, stride,
+                       (const W*)w, (const W*)b, rows, D, eps, d, (T*)y, stats);
+    return launch_status();
+}
+
+template <class T, class W>
+int launch_norm_bwd(const void* gy, const void* x, int64_t stride, const void* w, const float* stats, int64_t rows,
+                    int D, const Dropout& d, void* gx, void* gw, void* gb, hipStream_t st) {
+    if (gx && rows)
+        hipLaunchKernelGGL((k_norm_bwd_x<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kBlock), 0, st, (const T*)gy,
+                           (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx);
+    if (gw || gb)
+        hipLaunchKernelGGL((k_norm_bwd_w<T, W>), dim3(ceil_div(D, kWave)), dim3(kBlock), 0, st, (const T*)gy,
+                           (const T*)x, stride, stats, rows, D, d, (W*)gw, (W*)gb);
+    return launch_status();
+}
+
+// f<T, W>(args...) of the pair of types (norm_shape has refused the others)
+#define IGS_BY_TYPES(f, dtype, wdtype, ...)                                                             \
+    ((dtype) == IGS_F32   ? f<float, float>(__VA_ARGS__)                                                \
+     : (dtype) == IGS_F16 ? ((wdtype) == IGS_F32 ? f<f16, float>(__VA_ARGS__) : f<f16, f16>(__VA_ARGS__)) \
+                          : ((wdtype) == IGS_F32 ? f<bf16, float>(__VA_ARGS__) : f<bf16, bf16>(__VA_ARGS__)))
+// f<T, I>(args...) of an element type and a token width
+#define IGS_BY_TOKENS(f, dtype, bytes, ...)                                                            \
+    ((dtype) == IGS_F32   ? ((bytes) == 8 ? f<float, int64_t>(__VA_ARGS__) : f<float, int32_t>(__VA_ARGS__)) \
+     : (dtype) == IGS_F16 ? ((bytes) == 8 ? f<f16, int64_t>(__VA_ARGS__) : f<f16, int32_t>(__VA_ARGS__)) \
+                          : ((bytes) == 8 ? f<bf16, int64_t>(__VA_ARGS__) : f<bf16, int32_t>(__VA_ARGS__)))
+}  // namespace
+
+extern "C" {
+int igs_embedding_forward(const void* weight, int64_t weight_row_stride, int dtype, int64_t vocab, int D,
+                          const void* tokens, int token_bytes, int64_t count, float scale, void* out,
+                          igs_stream_t stream) {
+    if (!dtype_ok(dtype) || (token_bytes != 4 && token_bytes != 8)) return IGS_ERR_BAD_DTYPE;
+    const int rc = embedding_shape(vocab, D, count);
+    if (rc) return rc;
+    if (!isfinite(scale) || weight_row_stride < 0) return IGS_ERR_BAD_ARGUMENT;
+    if (count == 0) return IGS_OK;
+    if (!weight || !tokens || !out) return IGS_ERR_NULL_POINTER;
+    const int e = dtype_bytes(dtype);
+    if (!aligned_to(weight, e) || !aligned_to(out, e) || !aligned_to(tokens, token_bytes)) return IGS_ERR_ALIGNMENT;
+    return IGS_BY_TOKENS(launch_embed_fwd, dtype, token_bytes, weight, weight_row_stride, vocab, D, tokens, count,
+                         scale, out, (hipStream_t)stream);
+}
+
+int igs_embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding_plan_t* plan) {
+    return embedding_plan(vocab, D, dtype, count, plan);
+}
+
+int igs_embedding_backward(const void* grad_out, int dtype, const void* tokens, int token_bytes, int64_t count,
+                           int64_t vocab, int D, float scale, int64_t padding_idx, void* grad_weight, void* ws,
+                           size_t ws_bytes, igs_stream_t stream) {
+    if (token_bytes != 4 && token_bytes != 8) return IGS_ERR_BAD_DTYPE;
+    igs_embedding_plan_t p;
+    const int rc = embedding_plan(vocab, D, dtype, count, &p);
+    if (rc) return rc;
+    if (!isfinite(scale) || padding_idx < -1 || padding_idx >= vocab) return IGS_ERR_BAD_ARGUMENT;
+    if (!grad_weight || (count && (!grad_out || !tokens)) || (p.ws_bytes && !ws)) return IGS_ERR_NULL_POINTER;
+    if (ws_bytes < p.ws_bytes) return IGS_ERR_WORKSPACE;
+    const int e = dtype_bytes(dtype);
+    if (!aligned_to(ws, 16) || !aligned_to(grad_out, e) || !aligned_to(grad_weight, e) ||
+        !aligned_to(tokens, token_bytes))
+        return IGS_ERR_ALIGNMENT;
+    return IGS_BY_TOKENS(launch_embed_bwd, dtype, token_bytes, grad_out, tokens, count, vocab, D, scale, padding_idx,
+                         grad_weight, (hipStream_t)stream);
+}
+
+int igs_dropout(const void* x, int dtype, int64_t count, int threshold, uint64_t seed, const uint64_t* seed_device,
+                uint64_t offset, void* y, igs_stream_t stream) {
+    if (!dtype_ok(dtype)) return IGS_ERR_BAD_DTYPE;
+    if (count < 0 || count > (int64_t)1 << 50) return IGS_ERR_BAD_SHAPE;
+    Dropout d;
+    const int rc = make_dropout(threshold, seed, seed_device, offset, &d);
+    if (rc) return rc;
+    if (count == 0) return IGS_OK;
+    if (!x || !y) return IGS_ERR_NULL_POINTER;
+    const int e = dtype_bytes(dtype);
+    if (!aligned_to(x, e) || !aligned_to(y, e)) return IGS_ERR_ALIGNMENT;
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == IGS_F32   ? launch_dropout<float>(x, count, d, y, st)
+           : dtype == IGS_F16 ? launch_dropout<f16>(x, count, d, y, st)
+                              : launch_dropout<bf16>(x, count, d, y, st);
+}
+
+int igs_layer_norm_forward(const void* x, int64_t x_row_stride, int dtype, const void* weight, const void* bias,
+                           int wdtype, int64_t rows, int D, float eps, int threshold, uint64_t seed,
+                           const uint64_t* seed_device, uint64_t offset, void* y, float* stats, igs_stream_t stream) {
+    int rc = norm_shape(rows, D, dtype, wdtype);
+    if (rc) return rc;
+    if (!(eps >= 0.0f) || !isfinite(eps) || x_row_stride < 0) return IGS_ERR_BAD_ARGUMENT;
+    Dropout d;
+    rc = make_dropout(threshold, seed, seed_device, offset, &d);
+    if (rc) return rc;
+    if (rows == 0) return IGS_OK;
+    if (!x || !y) return IGS_ERR_NULL_POINTER;
+    const int e = dtype_bytes(dtype), we = dtype_bytes(wdtype);
+    if (!aligned_to(x, e) || !aligned_to(y, e) || !aligned_to(weight, we) || !aligned_to(bias, we) ||
+        !aligned_to(stats, 8))
+        return IGS_ERR_ALIGNMENT;
+    return IGS_BY_TYPES(launch_norm_fwd, dtype, wdtype, x, x_row_stride, weight, bias, rows, D, eps, d, y, stats,
+                        (hipStream_t)stream);
+}
+
+int igs_layer_norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* plan) {
+    return norm_plan(rows, D, dtype, wdtype, plan);
+}
+
+int igs_layer_norm_backward(const void* grad_y, const void* x, int64_t x_row_stride, int dtype, const void* weight,
+                            int wdtype, const float* stats, int64_t rows, int D, int threshold, uint64_t seed,
+                            const uint64_t* seed_device, uint64_t offset, void* grad_x, void* grad_weight,
+                            void* grad_bias, void* ws, size_t ws_bytes, igs_stream_t stream) {
+    igs_layer_norm_plan_t p;
+    int rc = norm_plan(rows, D, dtype, wdtype, &p);
+    if (rc) return rc;
+    if (x_row_stride < 0) return IGS_ERR_BAD_ARGUMENT;
+    Dropout d;
+    rc = make_dropout(threshold, seed, seed_device, offset, &d);
+    if (rc) return rc;
+    if (rows && (!grad_y || !x || !stats)) return IGS_ERR_NULL_POINTER;
+    if (p.ws_bytes && !ws && (grad_weight || grad_bias)) return IGS_ERR_NULL_POINTER;
+    if (ws_bytes < p.ws_bytes && (grad_weight || grad_bias)) return IGS_ERR_WORKSPACE;
+    const int e = dtype_bytes(dtype), we = dtype_bytes(wdtype);
+    if (!aligned_to(grad_y, e) || !aligned_to(x, e) || !aligned_to(grad_x, e) || !aligned_to(weight, we) ||
+        !aligned_to(grad_weight, we) || !aligned_to(grad_bias, we) || !aligned_to(stats, 8) || !aligned_to(ws, 16))
+        return IGS_ERR_ALIGNMENT;
+    return IGS_BY_TYPES(launch_norm_bwd, dtype, wdtype, grad_y, x, x_row_stride, weight, stats, rows, D, d, grad_x,
+                        grad_weight, grad_bias, (hipStream_t)stream);
+}
+}  // extern "C"

@@ -640,6 +640,8 @@ const char* igs_status_string(int status) {
         case IGS_ERR_ALIGNMENT: return "buffer not 16-byte aligned";
         case IGS_ERR_BAD_SKIP_WEIGHT: return "skip weight outside [0, 1)";
         case IGS_ERR_STATIC_SCRATCH: return "problem needs more scratch than the static array holds (IGS_STATIC_SCRATCH_BYTES)";
+        case IGS_ERR_BAD_DTYPE: return "unsupported element type or pair of types";
+        case IGS_ERR_BAD_ARGUMENT: return "argument outside its range";
         case IGS_ERR_STATIC_BUSY: return "the static scratch array is still in use by a call on another stream";
         default: break;
     }

@@ -19,7 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from . import _lib, _ops
+from . import _lib, _ops, feature as _feature
 from ._splat import KIND_COVINV, KIND_FEATURE, KIND_SCALE_ROT, channel_groups, run_backward, run_forward
 
 Tensor = torch.Tensor
@@ -260,9 +260,21 @@ class GaussianSplatting2D(nn.Module):
     `num_gaussians_per_emb` Gaussians (2 position, 2 log-scale, 1 rotation, 1 unused opacity
     logit, `output_dim` colours) per input feature, rendered by the fused HIP splat.
     Parameter names and init follow the reference (`proj.weight`, `proj.bias`), so its
-    checkpoints load."""
+    checkpoints load.
 
-    def __init__(self, num_gaussians_per_emb, emb_dim, output_dim=3, pos_map_offset=False):
+    Optional front of the head (none of it in the reference, whose `feature` comes as it is; without
+    these arguments the module, its parameters and its random draws are the reference's):
+      num_embeddings   a table `embedding.weight` [V, emb_dim]: `forward` then also takes token ids
+                       [B,F] (int32 or int64), looked up and multiplied by `emb_scale`; `padding_idx` is
+                       the row without a gradient
+      feature_norm     layer norm (`norm.weight`, `norm.bias`) of the features in front of `proj`
+      feature_dropout  probability of dropout in front of `proj` while training; a call's seed is drawn
+                       on the device from torch's generator, so `torch.manual_seed` governs it, and a
+                       captured graph draws a new one at each replay (`dropout_seed`, an int or an int64
+                       device tensor, is used instead when set)"""
+
+    def __init__(self, num_gaussians_per_emb, emb_dim, output_dim=3, pos_map_offset=False, num_embeddings=None,
+                 emb_scale=1.0, padding_idx=None, feature_norm=False, feature_dropout=0.0):
         super().__init__()
         self.num_gaussians_per_emb = num_gaussians_per_emb
         self.emb_dim = emb_dim
@@ -277,6 +289,13 @@ class GaussianSplatting2D(nn.Module):
         gaussian_bias[:, :2] = 0
         gaussian_bias[:, 2:4] = -4
         self.proj.bias.data.copy_(gaussian_bias.view_as(self.proj.bias))
+
+        _feature.dropout_threshold(feature_dropout)   # refuses a probability outside [0, 1]
+        self.emb_scale = float(emb_scale)
+        self.feature_dropout = float(feature_dropout)
+        self.dropout_seed = None
+        self.embedding = None if num_embeddings is None else nn.Embedding(num_embeddings, emb_dim, padding_idx)
+        self.norm = nn.LayerNorm(emb_dim) if feature_norm else None
 
     @staticmethod
     def xy_grid(size=None, device=None):
@@ -313,8 +332,29 @@ class GaussianSplatting2D(nn.Module):
         a, b, d = _cov_inverse_torch(scales, rotations, eps)
         return naive_gaussian_2d(x_grid, y_grid, positions, a, b, d, alphas, colors, eps)
 
+    def _head_input(self, feature, fused):
+        """Tokens or features -> what `proj` takes: lookup, norm and dropout where the module has them."""
+        if not feature.is_floating_point():
+            if self.embedding is None:
+                raise TypeError(f"feature must be floating point (the module has no embedding table); got {feature.dtype}")
+            lookup = _feature.embedding_lookup if fused else _feature.naive_embedding_lookup
+            feature = lookup(feature, self.embedding.weight, self.emb_scale, self.embedding.padding_idx)
+        p = self.feature_dropout if self.training else 0.0
+        seed = self.dropout_seed
+        if p and seed is None:
+            seed = torch.randint(0x7FFFFFFFFFFFFFFF, (1,), dtype=torch.int64, device=feature.device)
+        if self.norm is not None:
+            norm = _feature.layer_norm if fused else _feature.naive_layer_norm
+            return norm(feature, self.norm.weight, self.norm.bias, self.norm.eps, p, seed)
+        if p:
+            return (_feature.dropout if fused else _feature.naive_dropout)(feature, p, seed)
+        return feature
+
     def forward(self, feature, size=None, grid=None, pos_map=None, eps=1e-6, fused=True, scale=None):
-        """feature [B,F,D] -> (image [B,C,H,W], gs_feature [B,F*n,6+C]) (src/igs/gs2d.py:611-689)."""
+        """feature [B,F,D], or token ids [B,F] where the module has a table -> (image [B,C,H,W],
+        gs_feature [B,F*n,6+C]) (src/igs/gs2d.py:611-689)."""
+        if self.norm is not None or self.feature_dropout or not feature.is_floating_point():
+            feature = self._head_input(feature, fused)
         gs_feature = self.proj(feature).unflatten(-1, (-1, 6 + self.output_dim)).flatten(1, 2)
         b = gs_feature.shape[0]
 

@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define IGS_ABI_VERSION 8
+#define IGS_ABI_VERSION 9
 #define IGS_MAX_CHANNELS 16
 /* Size of the per-device static scratch array behind igs_gs2d_forward_static_ws. */
 #define IGS_STATIC_SCRATCH_BYTES (64u << 20)
@@ -45,8 +45,12 @@ typedef enum igs_status {
                                     IGS_STATIC_SCRATCH_BYTES */
     IGS_ERR_STATIC_BUSY = -10,   /* igs_gs2d_forward_static_ws: the previous call on this device, made on
                                     another stream, has not finished with the one scratch array */
-    IGS_ERR_BAD_SKIP_WEIGHT = -9 /* a pack call's skip_weight or skip_fraction is negative, NaN
+    IGS_ERR_BAD_SKIP_WEIGHT = -9, /* a pack call's skip_weight or skip_fraction is negative, NaN
                                     or >= 1 */
+    IGS_ERR_BAD_DTYPE = -11,     /* an element type outside igs_dtype, a pair of types that is not
+                                    compiled, or token ids of neither 4 nor 8 bytes */
+    IGS_ERR_BAD_ARGUMENT = -12   /* a number outside its range: an eps or scale that is not finite, a
+                                    dropout threshold outside 0..65536, a negative stride       */
 } igs_status;
 
 /* How the pixel coordinates are described.
@@ -432,6 +436,86 @@ int igs_koleo_forward(const float *features, int B, int N, int D, float *loss, v
  * through the normalisation).  grad_loss is one float of device memory. */
 int igs_koleo_backward(const void *saved, size_t saved_bytes, const float *grad_loss, int B, int N,
                        int D, float *grad_features, igs_stream_t stream);
+
+/* ---- Feature operators: what stands between tokens or features and the module's head -----------
+ * (the [B,F,D] input of src/igs/gs2d.py:611-635, whose `feature` the reference takes as given).
+ * Element types travel as igs_dtype; sums, means and norms are held in 32 bits, and every result
+ * is rounded once, to the type of its tensor. */
+typedef enum igs_dtype {
+    IGS_F32 = 0,
+    IGS_F16 = 1,
+    IGS_BF16 = 2
+} igs_dtype;
+
+/* Embedding lookup: out[i,:] = scale * weight[tokens[i],:], i < count.  weight: `vocab` rows of D
+ * elements, `weight_row_stride` elements apart; tokens: int32 or int64 (token_bytes 4 or 8),
+ * contiguous; out [count,D] contiguous in the type of weight.  A token outside [0, vocab) gives a
+ * row of NaN (nothing here waits for the device, so there is no status for it); count = 0 is a
+ * call without work.  1 <= vocab < 2^31 - 1, 1 <= D <= 2^20, 0 <= count < 2^31 - 1. */
+int igs_embedding_forward(const void *weight, int64_t weight_row_stride, int dtype, int64_t vocab,
+                          int D, const void *tokens, int token_bytes, int64_t count, float scale,
+                          void *out, igs_stream_t stream);
+
+/* Launch plan and workspace size of the dense gradient. */
+typedef struct igs_embedding_plan_t {
+    int64_t vocab, count;
+    int32_t D;
+    int32_t reserved;
+    uint64_t ws_bytes;       /* scratch of igs_embedding_backward                             */
+} igs_embedding_plan_t;
+
+int igs_embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding_plan_t *plan);
+
+/* Dense gradient of the lookup: grad_weight [vocab,D] (contiguous, every element written) =
+ * scale * sum over i with tokens[i] = v of grad_out[i,:], with the sum in 32 bits and a fixed order
+ * (bit-reproducible, no floating-point atomics); 0 for rows no token names, and for the row
+ * padding_idx (-1: none).  Tokens outside [0, vocab) contribute to nothing.  ws: plan.ws_bytes, 16-byte
+ * aligned, contents meaningless before and after. */
+int igs_embedding_backward(const void *grad_out, int dtype, const void *tokens, int token_bytes,
+                           int64_t count, int64_t vocab, int D, float scale, int64_t padding_idx,
+                           void *grad_weight, void *ws, size_t ws_bytes, igs_stream_t stream);
+
+/* Dropout from a counter-based generator; the mask is never stored.  Element i (its linear index)
+ * is dropped if its 16-bit number u_i < threshold (0..65536, i.e. 65536 p) and multiplied by
+ * 65536 / (65536 - threshold) otherwise; a dropped element is 0 whatever its value was.  u_i is half
+ * i % 2 (low half first) of 32-bit word (i % 8) / 2 of block i / 8 of Philox4x32 with seven rounds
+ * (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, 2011): counter words
+ * {block low, block high, offset low, offset high}, key {seed low, seed high}.  The seed is
+ * *seed_device when that is not NULL (8 bytes of device memory read by the kernel, so that a replayed
+ * graph sees what was written there since), else `seed`.  The same call on the upstream gradient is
+ * the backward. */
+int igs_dropout(const void *x, int dtype, int64_t count, int threshold, uint64_t seed,
+                const uint64_t *seed_device, uint64_t offset, void *y, igs_stream_t stream);
+
+/* Layer norm over rows of D elements, with dropout of its result when threshold > 0:
+ *   h = (x - mean) / sqrt(var + eps),  y = drop(h * weight + bias)
+ * x: `rows` rows, x_row_stride elements apart; y [rows,D] contiguous, same type (its linear index is
+ * the dropout index).  weight, bias [D] (either may be NULL: 1 and 0) of type wdtype, which is
+ * dtype or IGS_F32.  stats [rows][2] floats receives mean and 1 / sqrt(var + eps) for the backward
+ * (may be NULL).  1 <= D <= 2^20, 0 <= rows < 2^31 - 1. */
+int igs_layer_norm_forward(const void *x, int64_t x_row_stride, int dtype, const void *weight,
+                           const void *bias, int wdtype, int64_t rows, int D, float eps, int threshold,
+                           uint64_t seed, const uint64_t *seed_device, uint64_t offset, void *y,
+                           float *stats, igs_stream_t stream);
+
+typedef struct igs_layer_norm_plan_t {
+    int64_t rows;
+    int32_t D;
+    int32_t partials;        /* workgroups whose sums of the weight gradients are added at the end */
+    uint64_t ws_bytes;       /* scratch of igs_layer_norm_backward                             */
+} igs_layer_norm_plan_t;
+
+int igs_layer_norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t *plan);
+
+/* Gradients of igs_layer_norm_forward from its x and stats: with d = drop(grad_y) and g = d * weight,
+ *   grad_x = rstd (g - mean g - h mean(g h)),  grad_weight = sum_rows d h,  grad_bias = sum_rows d.
+ * grad_y, grad_x [rows,D] contiguous; grad_weight, grad_bias [D] of type wdtype.  Any of the three
+ * outputs may be NULL (not wanted).  The sums over rows have a fixed order (bit-reproducible). */
+int igs_layer_norm_backward(const void *grad_y, const void *x, int64_t x_row_stride, int dtype,
+                            const void *weight, int wdtype, const float *stats, int64_t rows, int D,
+                            int threshold, uint64_t seed, const uint64_t *seed_device, uint64_t offset,
+                            void *grad_x, void *grad_weight, void *grad_bias, void *ws, size_t ws_bytes,
+                            igs_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,257 @@
+"""Host side of the feature operators: refusals, plan arithmetic and status codes of the C ABI, shape functions, the
+module's options.  No kernel is launched, no GPU needed."""
+import ctypes
+
+import pytest
+import torch
+
+import igs_amd
+from igs_amd import _lib, feature
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from igs_amd import build
+
+    if build.is_stale():
+        build.build(verbose=False)
+    return _lib.load()
+
+
+def test_embedding_refusals():
+    w, t = torch.randn(5, 4), torch.tensor([1, 2])
+    with pytest.raises(RuntimeError, match="GPU only"):
+        igs_amd.embedding_lookup(t, w)
+    for bad in (torch.randn(5), torch.randn(0, 4), torch.randn(5, 0), torch.randn(2, 3, 4)):
+        with pytest.raises(ValueError, match=r"\[V, D\]"):
+            igs_amd.embedding_lookup(t, bad)
+    for bad in (t.float(), t.bool(), t.to(torch.int16), t.to(torch.uint8)):
+        with pytest.raises(TypeError, match="tokens"):
+            igs_amd.embedding_lookup(bad, w)
+    with pytest.raises(TypeError, match="weight"):
+        igs_amd.embedding_lookup(t, w.double())
+    for bad in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            igs_amd.embedding_lookup(t, w, bad)
+    for bad in (5, -6):
+        with pytest.raises(ValueError, match="padding_idx"):
+            igs_amd.embedding_lookup(t, w, padding_idx=bad)
+
+
+def test_layer_norm_refusals():
+    x = torch.randn(3, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        igs_amd.layer_norm(x)
+    for bad in (torch.tensor(1.0), torch.randn(3, 0)):
+        with pytest.raises(ValueError, match="last axis"):
+            igs_amd.layer_norm(bad)
+    with pytest.raises(TypeError, match="x must be"):
+        igs_amd.layer_norm(x.double())
+    for bad in (torch.randn(3), torch.randn(4, 1), torch.randn(4, 4)):
+        with pytest.raises(ValueError, match="weight"):
+            igs_amd.layer_norm(x, bad)
+        with pytest.raises(ValueError, match="bias"):
+            igs_amd.layer_norm(x, None, bad)
+    with pytest.raises(TypeError, match="weight"):
+        igs_amd.layer_norm(x, torch.ones(4, dtype=torch.int64))
+    for bad in (-1e-5, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            igs_amd.layer_norm(x, eps=bad)
+    with pytest.raises(ValueError, match="seed"):
+        igs_amd.layer_norm(x, dropout_p=0.5)
+
+
+def test_dropout_refusals():
+    x = torch.randn(3, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        igs_amd.dropout(x, 0.5, 1)
+    for bad in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="probability"):
+            igs_amd.dropout(x, bad, 1)
+    with pytest.raises(TypeError, match="x must be"):
+        igs_amd.dropout(x.double(), 0.5, 1)
+    for bad in (-1, 1 << 63):
+        with pytest.raises(ValueError, match=r"2\^63"):
+            igs_amd.dropout(x, 0.5, bad)
+        with pytest.raises(ValueError, match=r"2\^63"):
+            igs_amd.dropout(x, 0.5, 1, offset=bad)
+    for bad in (1.5, True, "1"):
+        with pytest.raises(TypeError, match="seed"):
+            igs_amd.dropout(x, 0.5, bad)
+    with pytest.raises(TypeError, match="offset"):
+        igs_amd.dropout(x, 0.5, 1, offset=1.0)
+    for bad in (torch.tensor([1, 2]), torch.tensor([1], dtype=torch.int32)):
+        with pytest.raises(TypeError, match="seed tensor"):
+            igs_amd.dropout(x, 0.5, bad)
+    with pytest.raises(RuntimeError, match="same device"):
+        igs_amd.dropout(torch.empty(3, device="meta"), 0.5, torch.tensor([1]))
+    assert igs_amd.dropout(x, 0.0, None) is x and igs_amd.dropout(x, 2.0 ** -18, 1) is x   # nothing is dropped
+    assert feature.dropout_threshold(1.0) == 65536 and feature.dropout_threshold(0.1) == 6554
+
+
+def test_mixed_devices_are_refused_before_any_launch():
+    """A host tensor beside a device tensor raises (a meta tensor stands for the other device: no GPU needed)."""
+    class Fake:
+        device = torch.device("cuda", 0)
+
+    with pytest.raises(RuntimeError, match="same device"):
+        feature._on_gpu(Fake, None, torch.zeros(2))
+
+
+def test_status_codes(lib):
+    """Arguments are rejected before anything is launched (4096 is never read)."""
+    p, E, N = ctypes.c_void_p(4096), _lib.EmbeddingPlan(), _lib.LayerNormPlan()
+    odd = ctypes.c_void_p(4097)
+    assert lib.igs_embedding_plan(10, 8, 0, 5, ctypes.byref(E)) == 0 and (E.vocab, E.D, E.count) == (10, 8, 5)
+    assert lib.igs_embedding_plan(10, 8, 0, 5, None) == -1
+    assert lib.igs_embedding_plan(10, 8, 3, 5, ctypes.byref(E)) == -11
+    for v, d, n in ((0, 8, 5), (10, 0, 5), (10, (1 << 20) + 1, 5), (10, 8, -1), (1 << 31, 8, 5), (10, 8, 1 << 31)):
+        assert lib.igs_embedding_plan(v, d, 0, n, ctypes.byref(E)) == -2
+    fwd = lib.igs_embedding_forward
+    assert fwd(p, 8, 0, 10, 8, p, 2, 5, 1.0, p, None) == -11
+    assert fwd(p, 8, 7, 10, 8, p, 4, 5, 1.0, p, None) == -11
+    assert fwd(p, -1, 0, 10, 8, p, 4, 5, 1.0, p, None) == -12
+    assert fwd(p, 8, 0, 10, 8, p, 4, 5, float("nan"), p, None) == -12
+    assert fwd(None, 8, 0, 10, 8, p, 4, 5, 1.0, p, None) == -1
+    assert fwd(odd, 8, 0, 10, 8, p, 4, 5, 1.0, p, None) == -7
+    assert fwd(None, 8, 0, 10, 8, None, 4, 0, 1.0, None, None) == 0         # no tokens: no work
+    bwd = lib.igs_embedding_backward
+    big = 1 << 40
+    assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, 10, p, p, big, None) == -12
+    assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, -2, p, p, big, None) == -12
+    assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, -1, None, p, big, None) == -1
+    assert bwd(p, 0, None, 8, 5, 10, 8, 1.0, -1, p, p, big, None) == -1
+    assert bwd(p, 0, odd, 8, 5, 10, 8, 1.0, -1, p, p, big, None) == -7
+    assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, -1, p, ctypes.c_void_p(4100), big, None) == -7
+    lib.igs_embedding_plan(10, 8, 0, 5, ctypes.byref(E))
+    if E.ws_bytes:
+        assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, -1, p, p, E.ws_bytes - 1, None) == -4
+        assert bwd(p, 0, p, 8, 5, 10, 8, 1.0, -1, p, None, big, None) == -1
+    d = lib.igs_dropout
+    assert d(p, 5, 8, 100, 0, None, 0, p, None) == -11 and d(p, 0, -1, 100, 0, None, 0, p, None) == -2
+    assert d(p, 0, 8, -1, 0, None, 0, p, None) == -12 and d(p, 0, 8, 65537, 0, None, 0, p, None) == -12
+    assert d(p, 0, 8, 100, 0, ctypes.c_void_p(4100), 0, p, None) == -7 and d(None, 0, 8, 100, 0, None, 0, p, None) == -1
+    assert d(odd, 1, 8, 100, 0, None, 0, p, None) == -7 and d(None, 0, 0, 100, 0, None, 0, None, None) == 0
+    assert lib.igs_layer_norm_plan(10, 8, 0, 0, ctypes.byref(N)) == 0 and (N.rows, N.D) == (10, 8)
+    assert lib.igs_layer_norm_plan(10, 8, 0, 0, None) == -1
+    assert lib.igs_layer_norm_plan(10, 8, 0, 1, ctypes.byref(N)) == -11     # fp32 rows with fp16 weights
+    assert lib.igs_layer_norm_plan(10, 8, 1, 2, ctypes.byref(N)) == -11
+    for r, D in ((-1, 8), (10, 0), (10, (1 << 20) + 1), (1 << 31, 8)):
+        assert lib.igs_layer_norm_plan(r, D, 0, 0, ctypes.byref(N)) == -2
+    f = lib.igs_layer_norm_forward
+    assert f(p, 8, 0, p, p, 0, 10, 8, -1.0, 0, 0, None, 0, p, p, None) == -12
+    assert f(p, -8, 0, p, p, 0, 10, 8, 1e-5, 0, 0, None, 0, p, p, None) == -12
+    assert f(p, 8, 0, p, p, 0, 10, 8, 1e-5, 70000, 0, None, 0, p, p, None) == -12
+    assert f(None, 8, 0, p, p, 0, 10, 8, 1e-5, 0, 0, None, 0, p, p, None) == -1
+    assert f(p, 8, 0, p, odd, 0, 10, 8, 1e-5, 0, 0, None, 0, p, p, None) == -7
+    assert f(p, 8, 0, p, p, 0, 10, 8, 1e-5, 0, 0, None, 0, p, ctypes.c_void_p(4100), None) == -7
+    assert f(None, 8, 0, p, p, 0, 0, 8, 1e-5, 0, 0, None, 0, None, None, None) == 0
+    b = lib.igs_layer_norm_backward
+    assert b(p, p, 8, 0, p, 0, None, 10, 8, 0, 0, None, 0, p, p, p, p, big, None) == -1
+    assert b(p, p, 8, 0, p, 0, p, 10, 8, -3, 0, None, 0, p, p, p, p, big, None) == -12
+    assert b(p, p, 8, 1, p, 2, p, 10, 8, 0, 0, None, 0, p, p, p, p, big, None) == -11
+    assert b(odd, p, 8, 0, p, 0, p, 10, 8, 0, 0, None, 0, p, p, p, p, big, None) == -7
+    lib.igs_layer_norm_plan(10, 8, 0, 0, ctypes.byref(N))
+    if N.ws_bytes:
+        assert b(p, p, 8, 0, p, 0, p, 10, 8, 0, 0, None, 0, p, p, p, p, N.ws_bytes - 1, None) == -4
+        assert b(p, p, 8, 0, p, 0, p, 10, 8, 0, 0, None, 0, p, p, p, None, big, None) == -1
+    assert b"element type" in lib.igs_status_string(-11) and b"range" in lib.igs_status_string(-12)
+
+
+def test_plan_structs_match_the_header():
+    import os
+    import re
+
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "igs_hip.h")).read()
+    for name, mirror in (("igs_embedding_plan_t", _lib.EmbeddingPlan), ("igs_layer_norm_plan_t", _lib.LayerNormPlan)):
+        body = re.sub(r"/\*.*?\*/", "", text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")], flags=re.S)
+        fields = []
+        for decl in body.split("{", 1)[1].split(";"):
+            if decl.strip():
+                typ, rest = decl.strip().split(None, 1)
+                fields += [(f.strip(), typ) for f in rest.split(",")]
+        want = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "uint64_t": ctypes.c_uint64}
+        assert [(n, want[t]) for n, t in fields] == list(mirror._fields_)
+
+
+def test_shape_functions():
+    """What torch.compile is told about the operators (meta tensors)."""
+    m = lambda *s, dtype=torch.bfloat16: torch.empty(*s, device="meta", dtype=dtype)
+    ops = torch.ops.igs_amd
+    t = m(2, 5, dtype=torch.int64)
+    y = ops.embedding_fwd(t, m(9, 16), 2.0, -1)
+    assert y.shape == (2, 5, 16) and y.dtype == torch.bfloat16
+    assert ops.embedding_bwd(y, t, 9, 2.0, -1).shape == (9, 16)
+    w = m(16, dtype=torch.float32)
+    y, stats = ops.layer_norm_fwd(m(2, 5, 16), w, None, 1e-5, 0, 0, None, 0)
+    assert y.shape == (2, 5, 16) and y.dtype == torch.bfloat16 and stats.shape == (10, 2) and stats.dtype == torch.float32
+    g = ops.layer_norm_bwd(y, m(2, 5, 16), w, None, stats, 0, 0, None, 0)
+    assert [(tuple(v.shape), v.dtype) for v in g] == [((2, 5, 16), torch.bfloat16), ((16,), torch.float32)]
+    assert ops.dropout(m(3, 7), 100, 1, None, 0).shape == (3, 7)
+
+
+@pytest.mark.parametrize("make,step", [
+    (lambda b: b, 24), (lambda b: b[..., :10], 24), (lambda b: b[:, ::2], 48), (lambda b: b[:, :1], 96),
+    (lambda b: b[:1, :1], 24), (lambda b: b.transpose(1, 2), None), (lambda b: b[..., ::2], None),
+    (lambda b: b[:1, :1].expand(7, 5, 24), 0), (lambda b: b[:, :1].expand(2, 4, 24), None), (lambda b: b[..., :1], 24),
+    (lambda b: b[:, :2], None)])
+def test_rows_taken_in_place(make, step):
+    """Rows that are dense and evenly spaced keep their memory; everything else is copied."""
+    v = make(torch.arange(2 * 4 * 24, dtype=torch.float32).view(2, 4, 24))
+    got, s = feature._rows(v)
+    if step is None:
+        assert got.is_contiguous() and s == v.shape[-1] and torch.equal(got, v)
+    else:
+        assert got is v
+        rows, D = v.numel() // v.shape[-1], v.shape[-1]
+        if rows > 1:
+            assert s == step
+        assert torch.equal(torch.as_strided(v, (rows, D), (s, 1)), v.reshape(rows, D))
+
+
+def test_module_defaults_are_unchanged_and_options_add_parameters():
+    torch.manual_seed(0)
+    a = igs_amd.GaussianSplatting2D(4, 32)
+    after = torch.rand(1)
+    assert sorted(a.state_dict()) == ["proj.bias", "proj.weight"]
+    torch.manual_seed(0)
+    b = igs_amd.GaussianSplatting2D(4, 32, num_embeddings=11, emb_scale=2.0, padding_idx=3, feature_norm=True,
+                                    feature_dropout=0.25)
+    assert sorted(b.state_dict()) == ["embedding.weight", "norm.bias", "norm.weight", "proj.bias", "proj.weight"]
+    assert torch.equal(a.proj.weight, b.proj.weight) and torch.equal(a.proj.bias, b.proj.bias)
+    torch.manual_seed(0)
+    igs_amd.GaussianSplatting2D(4, 32, feature_norm=True, feature_dropout=0.5)
+    assert torch.equal(torch.rand(1), after)           # no draw of its own without a table
+    with pytest.raises(ValueError, match="probability"):
+        igs_amd.GaussianSplatting2D(4, 32, feature_dropout=1.5)
+    with pytest.raises(TypeError, match="no embedding table"):
+        a(torch.zeros(2, 3, dtype=torch.int64), size=(4, 4))
+
+
+def test_module_debug_path_on_the_cpu():
+    """fused=False: lookup, norm and dropout as plain torch, then the plain splat; the mask is the operator's."""
+    torch.manual_seed(3)
+    m = igs_amd.GaussianSplatting2D(4, 16, num_embeddings=11, emb_scale=2.0, feature_norm=True, feature_dropout=0.25)
+    m.dropout_seed = 99
+    t = torch.randint(0, 11, (2, 5))
+    img, feat = m(t, size=(6, 7), fused=False)
+    f = m.embedding.weight[t] * 2.0
+    f = torch.nn.functional.layer_norm(f, (16,), m.norm.weight, m.norm.bias, m.norm.eps)
+    keep = igs_amd.dropout_keep_mask(f.shape, 0.25, 99)
+    plain = igs_amd.GaussianSplatting2D(4, 16)
+    plain.load_state_dict({k: v for k, v in m.state_dict().items() if k.startswith("proj")})
+    want_img, want_feat = plain(torch.where(keep, f / 0.75, torch.zeros_like(f)), size=(6, 7), fused=False)
+    assert torch.allclose(feat, want_feat, rtol=1e-5, atol=1e-6) and torch.allclose(img, want_img, rtol=1e-5, atol=1e-6)
+    img.sum().backward()
+    assert m.embedding.weight.grad is not None and m.norm.weight.grad is not None
+    m.eval()
+    a, b = m(t, size=(6, 7), fused=False)[0], m(t, size=(6, 7), fused=False)[0]
+    assert torch.equal(a, b)                             # no dropout in evaluation
+    m.train()
+    m.dropout_seed = None
+    assert not torch.equal(m(t, size=(6, 7), fused=False)[1], m(t, size=(6, 7), fused=False)[1])   # a new seed per call
+    torch.manual_seed(5)
+    a = m(t, size=(6, 7), fused=False)[1]
+    torch.manual_seed(5)
+    assert torch.equal(a, m(t, size=(6, 7), fused=False)[1])                                        # torch's generator governs it
+    m(torch.randn(2, 5, 16), size=(6, 7), fused=False)   # features still pass
