@@ -7,17 +7,26 @@ __device__ __forceinline__ bool token_ok(I t, int64_t vocab) {
     return (int64_t)t >= 0 && (int64_t)t < vocab;
 }
 
-// out[i,:] = scale * weight[tokens[i],:]; one element per thread.
-template <class T, class I>
+// out[i,:] = scale * weight[tokens[i],:].  `lanes` threads (a power of two, at most a workgroup) share a
+// token and walk its row in packs of V elements; the last pack of a row of another length is moved back
+// to end with the row.  Rows of fewer elements than a pack go with V = 1.
+template <class T, class I, int V>
 __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weight, int64_t stride, int64_t vocab,
                                                       int D, const I* __restrict__ tokens, int64_t count,
-                                                      float scale, T* __restrict__ out) {
-    const int64_t total = count * D, step = (int64_t)gridDim.x * kBlock;
-    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < total; e += step) {
-        const int64_t i = e / D;
+                                                      float scale, int lanes, T* __restrict__ out) {
+    const int per = kBlock / lanes, slot = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+    for (int64_t i = (int64_t)blockIdx.x * per + slot; i < count; i += (int64_t)gridDim.x * per) {
         const I t = tokens[i];
-        out[e] = token_ok(t, vocab) ? from_f32<T>(to_f32(weight[(int64_t)t * stride + (e - i * D)]) * scale)
-                                    : from_f32<T>(__builtin_nanf(""));
+        const bool ok = token_ok(t, vocab);
+        const T* src = weight + (ok ? (int64_t)t : 0) * stride;
+        T* dst = out + i * D;
+        for (int d = lane * V; d < D; d += lanes * V) {
+            const int at = d + V <= D ? d : D - V;
+            Pack<T, V> q = load_pack<T, V>(src + at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) q.v[j] = ok ? from_f32<T>(to_f32(q.v[j]) * scale) : from_f32<T>(__builtin_nanf(""));
+            store_pack<T, V>(dst + at, q);
+        }
     }
 }
 

@@ -11,6 +11,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "igs_hip.h"
 
 namespace {
@@ -70,23 +72,89 @@ int norm_shape(int64_t rows, int D, int dtype, int wdtype) {
     return IGS_OK;
 }
 
+// Compute units of the current device (of an MI355X where there is none: plans are made without a GPU too).
+int device_cus() {
+    static std::atomic<int> cached{0};
+    int cus = cached.load(std::memory_order_relaxed);
+    if (cus > 0) return cus;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    cached.store(cus, std::memory_order_relaxed);
+    return cus;
+}
+
+// How a row of D elements is laid over threads: TPR threads of NV packs of V elements.  The smallest
+// arrangement that holds the row: 16 elements per thread at most (more would cost the backward its
+// occupancy: x, gy, h, d, w and the two sums of every element are in registers).
+struct NormShape {
+    int tpr, nv;
+    bool one, is_long;  // V = 1; no arrangement holds the row
+};
+
+NormShape norm_layout(int D, int dtype) {
+    const int V = 16 / dtype_bytes(dtype);
+    if (D < V) return {8, 1, true, false};
+    const int packs = (int)ceil_div(D, V);
+    const int most = 16 / V;  // packs per thread
+    for (int tpr = 8; tpr <= kWave; tpr *= 2)
+        if (packs <= tpr) return {tpr, 1, false, false};
+    for (int tpr = kWave; tpr <= 1024; tpr *= 4)
+        for (int nv = tpr == kWave ? 2 : most / 2; nv <= most; nv *= 2)
+            if (packs <= tpr * nv) return {tpr, nv, false, false};
+    return {1024, 0, false, true};
+}
+
+inline int norm_rows_at_once(const NormShape& s) { return s.tpr > kBlock ? 1 : kBlock / s.tpr; }
+
+#ifndef IGS_NORM_FWD_WGS
+#define IGS_NORM_FWD_WGS 8
+#endif
+#ifndef IGS_NORM_BWD_WGS
+#define IGS_NORM_BWD_WGS 4
+#endif
+// Workgroups of the norm kernels: resident at once where there are more rows than that.
+int64_t norm_groups(const NormShape& s, int64_t rows, int per_cu) {
+    const int64_t all = ceil_div(rows, norm_rows_at_once(s));
+    return at_most(all, (int64_t)device_cus() * (s.tpr > kBlock ? (per_cu + 3) / 4 : per_cu));
+}
+
 int norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* p) {
     if (!p) return IGS_ERR_NULL_POINTER;
     const int rc = norm_shape(rows, D, dtype, wdtype);
     if (rc) return rc;
+    const NormShape s = norm_layout(D, dtype);
+    int64_t P;
+    if (s.is_long) {  // row groups so that there are eight workgroups per compute unit
+        P = ceil_div((int64_t)device_cus() * 8, ceil_div(D, kWave));
+        P = at_most(P, ceil_div(rows, kBlock / kWave));
+    } else {
+        P = norm_groups(s, rows, IGS_NORM_BWD_WGS);
+    }
     p->rows = rows;
     p->D = D;
-    p->partials = 0;
-    p->ws_bytes = 0;
+    p->partials = (int32_t)P;
+    p->ws_bytes = (uint64_t)P * 2 * D * sizeof(float);
     return IGS_OK;
 }
 
 template <class T, class I>
 int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, const void* tokens, int64_t count,
                      float scale, void* out, hipStream_t st) {
-    const int64_t blocks = at_most(ceil_div(count * D, kBlock), 1 << 20);
-    hipLaunchKernelGGL((k_embed_fwd<T, I>), dim3(blocks), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
-                       (const I*)tokens, count, scale, (T*)out);
+    constexpr int V = kVec<T>;
+    const int packs = D < V ? D : (int)ceil_div(D, V);
+    int lanes = 1;
+    while (lanes < packs && lanes < kBlock) lanes *= 2;
+    const int64_t groups = at_most(ceil_div(count, kBlock / lanes), 1 << 20);
+    if (D < V)
+        hipLaunchKernelGGL((k_embed_fwd<T, I, 1>), dim3(groups), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
+                           (const I*)tokens, count, scale, lanes, (T*)out);
+    else
+        hipLaunchKernelGGL((k_embed_fwd<T, I, V>), dim3(groups), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
+                           (const I*)tokens, count, scale, lanes, (T*)out);
     return launch_status();
 }
 
@@ -100,28 +168,79 @@ int launch_embed_bwd(const void* grad, const void* tokens, int64_t count, int64_
 
 template <class T>
 int launch_dropout(const void* x, int64_t count, const Dropout& d, void* y, hipStream_t st) {
-    const int64_t blocks = at_most(ceil_div(ceil_div(count, 8), kBlock), 1 << 20);
-    hipLaunchKernelGGL((k_dropout<T>), dim3(blocks), dim3(kBlock), 0, st, (const T*)x, count, d, (T*)y);
+    constexpr int kPacks = 2;
+    const int64_t packs = count / kVec<T>, groups = packs ? ceil_div(packs, kBlock * kPacks) : 1;
+    hipLaunchKernelGGL((k_dropout<T, kPacks>), dim3(groups), dim3(kBlock), 0, st, (const T*)x, count, d, (T*)y);
     return launch_status();
+}
+
+// f(TPR, NV, V) as constants for the arrangement `s` of a row
+template <int TPR, int NV, int V>
+struct NormLayout {
+    static constexpr int tpr = TPR, nv = NV, v = V;
+};
+template <class T, class F>
+void norm_dispatch(const NormShape& s, F f) {
+    constexpr int V = kVec<T>, kMost = 16 / V;
+    if (s.one) return f(NormLayout<8, 1, 1>());
+    if (s.nv == 1 && s.tpr <= kWave) {
+        if (s.tpr == 8) return f(NormLayout<8, 1, V>());
+        if (s.tpr == 16) return f(NormLayout<16, 1, V>());
+        if (s.tpr == 32) return f(NormLayout<32, 1, V>());
+        return f(NormLayout<64, 1, V>());
+    }
+    if (s.tpr == kWave) {
+        if (s.nv == 2) return f(NormLayout<64, 2, V>());
+        return f(NormLayout<64, kMost, V>());
+    }
+    if (s.tpr == 256) {
+        if (s.nv == kMost / 2) return f(NormLayout<256, kMost / 2, V>());
+        return f(NormLayout<256, kMost, V>());
+    }
+    if (s.nv == kMost / 2) return f(NormLayout<1024, kMost / 2, V>());
+    return f(NormLayout<1024, kMost, V>());
 }
 
 template <class T, class W>
 int launch_norm_fwd(const void* x, int64_t stride, const void* w, const void* b, int64_t rows, int D, float eps,
                     const Dropout& d, void* y, float* stats, hipStream_t st) {
-    hipLaunchKernelGGL((k_norm_fwd<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kBlock), 0, st, (const T*)x, stride,
-                       (const W*)w, (const W*)b, rows, D, eps, d, (T*)y, stats);
+    const NormShape s = norm_layout(D, sizeof(T) == 4 ? IGS_F32 : IGS_F16);
+    if (s.is_long)
+        hipLaunchKernelGGL((k_norm_fwd_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)x, stride,
+                           (const W*)w, (const W*)b, rows, D, eps, d, (T*)y, stats);
+    else
+        norm_dispatch<T>(s, [&](auto l) {
+            using L = decltype(l);
+            hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v>), dim3(norm_groups(s, rows, IGS_NORM_FWD_WGS)),
+                               dim3(norm_threads(L::tpr)), 0, st, (const T*)x, stride, (const W*)w, (const W*)b, rows, D,
+                               eps, d, (T*)y, stats);
+        });
     return launch_status();
 }
 
 template <class T, class W>
 int launch_norm_bwd(const void* gy, const void* x, int64_t stride, const void* w, const float* stats, int64_t rows,
-                    int D, const Dropout& d, void* gx, void* gw, void* gb, hipStream_t st) {
-    if (gx && rows)
-        hipLaunchKernelGGL((k_norm_bwd_x<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kBlock), 0, st, (const T*)gy,
-                           (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx);
-    if (gw || gb)
-        hipLaunchKernelGGL((k_norm_bwd_w<T, W>), dim3(ceil_div(D, kWave)), dim3(kBlock), 0, st, (const T*)gy,
-                           (const T*)x, stride, stats, rows, D, d, (W*)gw, (W*)gb);
+                    int D, const Dropout& d, int partials, void* gx, void* gw, void* gb, float* part, hipStream_t st) {
+    const NormShape s = norm_layout(D, sizeof(T) == 4 ? IGS_F32 : IGS_F16);
+    const bool sums = gw || gb;
+    if (rows && s.is_long) {
+        if (gx)
+            hipLaunchKernelGGL((k_norm_bwd_x_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)gy,
+                               (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx);
+        if (sums)
+            hipLaunchKernelGGL((k_norm_bwd_w_long<T>), dim3(ceil_div(D, kWave), partials), dim3(kBlock), 0, st,
+                               (const T*)gy, (const T*)x, stride, stats, rows, D, d, part);
+    } else if (rows && (gx || sums)) {
+        norm_dispatch<T>(s, [&](auto l) {
+            using L = decltype(l);
+            hipLaunchKernelGGL((k_norm_bwd<T, W, L::tpr, L::nv, L::v>), dim3(partials), dim3(norm_threads(L::tpr)), 0, st,
+                               (const T*)gy, (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx,
+                               sums ? part : (float*)nullptr);
+        });
+    }
+    if (sums)
+        hipLaunchKernelGGL((k_norm_reduce<W>), dim3(ceil_div(2 * D, kWave)), dim3(kWave * kReduceWaves), 0, st,
+                           (const float*)part, partials, D, (W*)gw, (W*)gb);
     return launch_status();
 }
 
@@ -178,7 +297,7 @@ int igs_embedding_backward(const void* grad_out, int dtype, const void* tokens, 
 int igs_dropout(const void* x, int dtype, int64_t count, int threshold, uint64_t seed, const uint64_t* seed_device,
                 uint64_t offset, void* y, igs_stream_t stream) {
     if (!dtype_ok(dtype)) return IGS_ERR_BAD_DTYPE;
-    if (count < 0 || count > (int64_t)1 << 50) return IGS_ERR_BAD_SHAPE;
+    if (count < 0 || count >= (int64_t)1 << 34) return IGS_ERR_BAD_SHAPE;
     Dropout d;
     const int rc = make_dropout(threshold, seed, seed_device, offset, &d);
     if (rc) return rc;
@@ -233,7 +352,7 @@ int igs_layer_norm_backward(const void* grad_y, const void* x, int64_t x_row_str
     if (!aligned_to(grad_y, e) || !aligned_to(x, e) || !aligned_to(grad_x, e) || !aligned_to(weight, we) ||
         !aligned_to(grad_weight, we) || !aligned_to(grad_bias, we) || !aligned_to(stats, 8) || !aligned_to(ws, 16))
         return IGS_ERR_ALIGNMENT;
-    return IGS_BY_TYPES(launch_norm_bwd, dtype, wdtype, grad_y, x, x_row_stride, weight, stats, rows, D, d, grad_x,
-                        grad_weight, grad_bias, (hipStream_t)stream);
+    return IGS_BY_TYPES(launch_norm_bwd, dtype, wdtype, grad_y, x, x_row_stride, weight, stats, rows, D, d, p.partials,
+                        grad_x, grad_weight, grad_bias, (float*)ws, (hipStream_t)stream);
 }
 }  // extern "C"

@@ -1,6 +1,6 @@
-// igs_feature_common.h -- element types, conversions and the counter-based generator shared by the
-// feature operators (embedding lookup, layer norm, dropout).  Included by igs_feature.hip inside its
-// anonymous namespace.
+// igs_feature_common.h -- element types, wide loads, sums across lanes and the counter-based generator
+// shared by the feature operators (embedding lookup, layer norm, dropout).  Included by igs_feature.hip
+// inside its anonymous namespace.
 #pragma once
 
 constexpr int kWave = 64;
@@ -17,6 +17,47 @@ __device__ __forceinline__ float to_f32(T v) {
 template <class T>
 __device__ __forceinline__ T from_f32(float v) {
     return (T)v;
+}
+
+// Elements of one 16-byte access.  A Pack has its element's alignment: global memory takes a 16-byte
+// access at any address, so rows of odd lengths and misaligned views go the same way as others.
+template <class T>
+constexpr int kVec = 16 / (int)sizeof(T);
+template <class T, int V>
+struct Pack {
+    T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& q) {
+    *reinterpret_cast<Pack<T, V>*>(p) = q;
+}
+
+// Sums over the TPR lanes of a row within a wave (TPR = 8, 16, 32 or 64), the same bits in all of them.
+// Every lane of the wave takes part.  Data-parallel moves inside 16 lanes; a whole wave's four sums
+// of 16 are read as scalars.
+template <int kCtrl>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true));
+}
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+    static_assert(TPR == 8 || TPR == 16 || TPR == 32 || TPR == 64, "");
+    v = dpp_add<0xB1>(v);   // lane ^ 1
+    v = dpp_add<0x4E>(v);   // lane ^ 2
+    v = dpp_add<0x141>(v);  // mirrored within 8
+    if (TPR >= 16) v = dpp_add<0x140>(v);  // mirrored within 16
+    if (TPR == 32) v += __shfl_xor(v, 16);
+    if (TPR == 64) {
+        const int i = __float_as_int(v);
+        const float a = __int_as_float(__builtin_amdgcn_readlane(i, 0)), b = __int_as_float(__builtin_amdgcn_readlane(i, 16));
+        const float c = __int_as_float(__builtin_amdgcn_readlane(i, 32)), d = __int_as_float(__builtin_amdgcn_readlane(i, 48));
+        v = (a + b) + (c + d);
+    }
+    return v;
 }
 
 // What a call's dropout needs: the keep rule, the factor of what stays, and the generator's state.
@@ -66,4 +107,36 @@ __device__ __forceinline__ void philox(uint64_t block, const PhiloxKey& key, uin
 // Number of element `j` (0..7) of a block.
 __device__ __forceinline__ uint32_t philox_u16(const uint32_t (&w)[4], int j) {
     return (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
+}
+// Bit j: element j of the block stays.
+__device__ __forceinline__ uint32_t keep_bits(uint64_t block, const Dropout& d, const PhiloxKey& key) {
+    uint32_t w[4], bits = 0;
+    philox(block, key, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits |= (philox_u16(w, j) >= d.threshold ? 1u : 0u) << j;
+    return bits;
+}
+
+// v = dropped ? 0 : v * factor for V consecutive elements from linear index `first`.  `whole`
+// (wave-uniform): every row length is a multiple of 8, so first is a multiple of V and the elements lie
+// in one block; otherwise they may reach into the next one.
+template <int V>
+__device__ __forceinline__ void drop(float (&v)[V], uint64_t first, bool whole, const Dropout& d, const PhiloxKey& key) {
+    if (V > 1 && whole) {
+        uint32_t w[4];
+        philox(first >> 3, key, w);
+        if (V == 4 && (first & 4)) {
+            w[0] = w[2];
+            w[1] = w[3];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = philox_u16(w, j & 7) >= d.threshold ? v[j] * d.factor : 0.0f;
+    } else {
+        const uint32_t shift = (uint32_t)(first & 7);
+        uint32_t bits = keep_bits(first >> 3, d, key);
+        if (shift + V > 8) bits |= keep_bits((first >> 3) + 1, d, key) << 8;
+        bits >>= shift;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (bits >> j) & 1 ? v[j] * d.factor : 0.0f;
+    }
 }

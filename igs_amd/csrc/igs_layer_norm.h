@@ -1,51 +1,348 @@
 // igs_layer_norm.h -- layer norm over rows, forward and backward, with dropout of its result.
 // Included by igs_feature.hip inside its anonymous namespace.
+//
+//   h = (x - mean) rstd,  y = drop(h w + b);   d = drop(gy), g = d w
+//   gx = rstd (g - mean g - h mean(g h)),  gw = sum_rows d h,  gb = sum_rows d
+//
+// Bound by memory: a row is read once and stays in registers between its sums and its result.  TPR
+// threads share a row (8 to 64 lanes of a wave, or a workgroup of 256 or 1024 threads), NV packs of 16
+// bytes each; the weights of a thread's columns stay in registers while its workgroup walks over the
+// rows, the next row's loads in flight.  The last pack of a row whose length is no multiple of the
+// pack is moved back to end with the row: its first elements are the neighbour's (computed twice, counted
+// once).  The backward keeps the two sums over rows for a thread's columns in registers; each workgroup
+// leaves one partial row of them, and k_norm_reduce adds those in a fixed order.
 #pragma once
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
+// Sum of up to two values over the TPR threads of a row; `red` as two buffers used in turn, so that one barrier per
+// sum is enough (a wave can be at most one sum ahead of another).
+template <int TPR>
+struct RowSum {
+    static constexpr int kWaves = TPR / kWave;
+    float (*red)[2][kWaves > 0 ? kWaves : 1];
+    int turn;
+
+    __device__ __forceinline__ void operator()(float& a, float& b) {
+        if constexpr (TPR <= kWave) {
+            a = lanes_sum<TPR>(a);
+            b = lanes_sum<TPR>(b);
+        } else {
+            a = lanes_sum<kWave>(a);
+            b = lanes_sum<kWave>(b);
+            if ((threadIdx.x & (kWave - 1)) == 0) {
+                red[turn][0][threadIdx.x / kWave] = a;
+                red[turn][1][threadIdx.x / kWave] = b;
+            }
+            __syncthreads();
+            a = b = 0.0f;
 #pragma unroll
-    for (int k = kWave / 2; k > 0; k >>= 1) v += __shfl_xor(v, k);
-    __syncthreads();  // the previous sum has been read
-    if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = v;
-    __syncthreads();
+            for (int w = 0; w < kWaves; ++w) {
+                a += red[turn][0][w];
+                b += red[turn][1][w];
+            }
+            turn ^= 1;
+        }
+    }
+    __device__ __forceinline__ void operator()(float& a) {
+        if constexpr (TPR <= kWave) {
+            a = lanes_sum<TPR>(a);
+        } else {
+            a = lanes_sum<kWave>(a);
+            if ((threadIdx.x & (kWave - 1)) == 0) red[turn][0][threadIdx.x / kWave] = a;
+            __syncthreads();
+            a = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) a += red[turn][0][w];
+            turn ^= 1;
+        }
+    }
+};
+
+constexpr int norm_threads(int tpr) { return tpr > kBlock ? tpr : kBlock; }
+
+template <class T, class W, int TPR, int NV, int V>
+__global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restrict__ x, int64_t stride,
+                                                                const W* __restrict__ w, const W* __restrict__ b,
+                                                                int64_t rows, int D, float eps, Dropout drop_,
+                                                                T* __restrict__ y, float* __restrict__ stats) {
+    constexpr int kRows = norm_threads(TPR) / TPR;  // rows of a workgroup at a time
+    __shared__ float red[2][2][TPR > kWave ? TPR / kWave : 1];
+    RowSum<TPR> row_sum{red, 0};
+    const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    const PhiloxKey key = philox_key(drop_);
+    const bool whole = D % 8 == 0, ragged = D % V != 0;
+    const float inv = 1.0f / (float)D;
+
+    int start[NV], skip[NV];  // first element of a pack, elements of it that another thread counts (V: no pack)
+    float wv[NV][V], bv[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int col = (k * TPR + lane) * V;
+        start[k] = col + V <= D ? col : D - V;
+        skip[k] = col < D ? col - start[k] : V;
+        Pack<W, V> pw, pb;
+        if (skip[k] < V) {
+            if (w) pw = load_pack<W, V>(w + start[k]);
+            if (b) pb = load_pack<W, V>(b + start[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            wv[k][j] = w ? to_f32(pw.v[j]) : 1.0f;
+            bv[k][j] = b ? to_f32(pb.v[j]) : 0.0f;
+        }
+    }
+
+    Pack<T, V> next[NV];
+    int64_t r0 = (int64_t)blockIdx.x * kRows;
+    const auto load = [&](int64_t first) {
+        const int64_t r = first + slot < rows ? first + slot : rows - 1;  // a slot behind the last row computes it again
+        const T* p = x + r * stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (skip[k] < V) next[k] = load_pack<T, V>(p + start[k]);
+    };
+    if (r0 < rows) load(r0);
+    for (; r0 < rows; r0 += step) {
+        float c[NV][V];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[k][j] = skip[k] < V ? to_f32(next[k].v[j]) : 0.0f;
+        if (r0 + step < rows) load(r0 + step);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += !ragged || j >= skip[k] ? c[k][j] : 0.0f;
+        row_sum(s);
+        const float mean = s * inv;
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                c[k][j] -= mean;
+                s = fmaf(c[k][j], j >= skip[k] ? c[k][j] : 0.0f, s);
+            }
+        row_sum(s);
+        const float rstd = 1.0f / sqrtf(fmaf(s, inv, eps));
+        const int64_t r = r0 + slot;
+        if (r < rows) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (skip[k] < V) {
+                    Pack<T, V> q;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) c[k][j] = fmaf(c[k][j] * rstd, wv[k][j], bv[k][j]);
+                    if (drop_.threshold) drop<V>(c[k], (uint64_t)r * D + start[k], whole, drop_, key);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(c[k][j]);
+                    store_pack<T, V>(y + r * D + start[k], q);
+                }
+            if (stats && lane == 0) {
+                stats[2 * r] = mean;
+                stats[2 * r + 1] = rstd;
+            }
+        }
+    }
+}
+
+// part [gridDim.x][2][D]: a workgroup's sums over its rows of d h and of d.  gx may be NULL, and part where neither sum
+// is wanted.
+template <class T, class W, int TPR, int NV, int V>
+__global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restrict__ gy, const T* __restrict__ x,
+                                                                int64_t stride, const W* __restrict__ w,
+                                                                const float* __restrict__ stats, int64_t rows, int D,
+                                                                Dropout drop_, T* __restrict__ gx,
+                                                                float* __restrict__ part) {
+    constexpr int kRows = norm_threads(TPR) / TPR;
+    __shared__ float red[2][2][TPR > kWave ? TPR / kWave : 1];
+    __shared__ float sums[TPR <= kWave ? 2 * TPR * NV * V : 1];
+    RowSum<TPR> row_sum{red, 0};
+    const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    const PhiloxKey key = philox_key(drop_);
+    const bool whole = D % 8 == 0;
+    const float inv = 1.0f / (float)D;
+
+    int start[NV], skip[NV];
+    float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int col = (k * TPR + lane) * V;
+        start[k] = col + V <= D ? col : D - V;
+        skip[k] = col < D ? col - start[k] : V;
+        Pack<W, V> pw;
+        if (w && skip[k] < V) pw = load_pack<W, V>(w + start[k]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            wv[k][j] = w ? to_f32(pw.v[j]) : 1.0f;
+            aw[k][j] = ab[k][j] = 0.0f;
+        }
+    }
+
+    Pack<T, V> nx[NV], ng[NV];
+    float2 ns;
+    const auto load = [&](int64_t first) {
+        const int64_t r = first + slot < rows ? first + slot : rows - 1;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (skip[k] < V) {
+                nx[k] = load_pack<T, V>(x + r * stride + start[k]);
+                ng[k] = load_pack<T, V>(gy + r * D + start[k]);
+            }
+        ns = reinterpret_cast<const float2*>(stats)[r];
+    };
+    int64_t r0 = (int64_t)blockIdx.x * kRows;
+    if (r0 < rows) load(r0);
+    for (; r0 < rows; r0 += step) {
+        float h[NV][V], d[NV][V];
+        const float mean = ns.x, rstd = ns.y;
+        const int64_t r = r0 + slot;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[k][j] = skip[k] < V ? (to_f32(nx[k].v[j]) - mean) * rstd : 0.0f;
+                d[k][j] = skip[k] < V && r < rows ? to_f32(ng[k].v[j]) : 0.0f;
+            }
+            if (drop_.threshold) drop<V>(d[k], (uint64_t)r * D + start[k], whole, drop_, key);
+        }
+        if (r0 + step < rows) load(r0 + step);
+        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                aw[k][j] = fmaf(d[k][j], h[k][j], aw[k][j]);
+                ab[k][j] += d[k][j];
+                d[k][j] *= wv[k][j];
+                const float g = j >= skip[k] ? d[k][j] : 0.0f;
+                s0 += g;
+                s1 = fmaf(g, h[k][j], s1);
+            }
+        if (!gx) continue;  // uniform
+        row_sum(s0, s1);
+        s0 *= inv;
+        s1 *= inv;
+        if (r < rows) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (skip[k] < V) {
+                    Pack<T, V> q;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(rstd * (d[k][j] - fmaf(h[k][j], s1, s0)));
+                    store_pack<T, V>(gx + r * D + start[k], q);
+                }
+        }
+    }
+    if (!part) return;
+    float* out = part + (size_t)blockIdx.x * 2 * D;
+    if constexpr (TPR > kWave) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j >= skip[k]) {
+                    out[start[k] + j] = aw[k][j];
+                    out[D + start[k] + j] = ab[k][j];
+                }
+    } else {
+        // rows of one wave by lane exchange, then the four waves one after the other
+#pragma unroll
+        for (int m = TPR; m < kWave; m <<= 1)
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    aw[k][j] += __shfl_xor(aw[k][j], m);
+                    ab[k][j] += __shfl_xor(ab[k][j], m);
+                }
+        const int wave = threadIdx.x / kWave, at = threadIdx.x & (kWave - 1);
+        for (int q = 0; q < kBlock / kWave; ++q) {
+            if (wave == q && at < TPR) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        float* p = sums + ((k * V + j) * TPR + at) * 2;
+                        p[0] = q ? p[0] + aw[k][j] : aw[k][j];
+                        p[1] = q ? p[1] + ab[k][j] : ab[k][j];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave == 0 && at < TPR) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j >= skip[k]) {
+                        const float* p = sums + ((k * V + j) * TPR + at) * 2;
+                        out[start[k] + j] = p[0];
+                        out[D + start[k] + j] = p[1];
+                    }
+        }
+    }
+}
+
+// gw, gb = the column sums of part [P][2][D].  A workgroup owns 64 of the 2 D columns; each of its 16 waves adds every
+// sixteenth partial row.
+constexpr int kReduceWaves = 16;
+template <class W>
+__global__ __launch_bounds__(kWave* kReduceWaves) void k_norm_reduce(const float* __restrict__ part, int P, int D,
+                                                                     W* __restrict__ gw, W* __restrict__ gb) {
+    __shared__ float red[kReduceWaves][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int col = blockIdx.x * kWave + lane;
     float s = 0.0f;
+    if (col < 2 * D) {
+#pragma unroll 8
+        for (int p = wave; p < P; p += kReduceWaves) s += part[(size_t)p * 2 * D + col];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < 2 * D) {
+        s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kBlock / kWave; ++w) s += red[w];
-    return s;
+        for (int k = 0; k < kReduceWaves; ++k) s += red[k][lane];
+        if (col < D) {
+            if (gw) gw[col] = from_f32<W>(s);
+        } else if (gb) {
+            gb[col - D] = from_f32<W>(s);
+        }
+    }
 }
 
-__device__ __forceinline__ float drop_one(float v, int64_t i, const Dropout& drop, const PhiloxKey& key) {
-    if (drop.threshold == 0) return v;
-    uint32_t w[4];
-    philox((uint64_t)(i >> 3), key, w);
-    const uint32_t pair = (i & 4) ? ((i & 2) ? w[3] : w[2]) : ((i & 2) ? w[1] : w[0]);
-    const uint32_t u = (i & 1) ? pair >> 16 : pair & 0xFFFFu;
-    return u >= drop.threshold ? v * drop.factor : 0.0f;
-}
+// ---- rows that do not fit a workgroup's registers: read again for every step -------------------------
+constexpr int kLong = 1024;
 
-// One workgroup per row: mean, then the sum of squared deviations, then the result.
 template <class T, class W>
-__global__ __launch_bounds__(kBlock) void k_norm_fwd(const T* __restrict__ x, int64_t stride,
-                                                     const W* __restrict__ w, const W* __restrict__ b, int64_t rows,
-                                                     int D, float eps, Dropout drop, T* __restrict__ y,
-                                                     float* __restrict__ stats) {
-    __shared__ float red[kBlock / kWave];
-    const PhiloxKey key = philox_key(drop);
+__global__ __launch_bounds__(kLong) void k_norm_fwd_long(const T* __restrict__ x, int64_t stride,
+                                                         const W* __restrict__ w, const W* __restrict__ b,
+                                                         int64_t rows, int D, float eps, Dropout drop_,
+                                                         T* __restrict__ y, float* __restrict__ stats) {
+    __shared__ float red[2][2][kLong / kWave];
+    RowSum<kLong> row_sum{red, 0};
+    const PhiloxKey key = philox_key(drop_);
+    const float inv = 1.0f / (float)D;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + r * stride;
         float s = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kBlock) s += to_f32(xr[d]);
-        const float mean = block_sum(s, red) / (float)D;
+        for (int d = threadIdx.x; d < D; d += kLong) s += to_f32(xr[d]);
+        row_sum(s);
+        const float mean = s * inv;
         s = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kBlock) {
+        for (int d = threadIdx.x; d < D; d += kLong) {
             const float c = to_f32(xr[d]) - mean;
             s = fmaf(c, c, s);
         }
-        const float rstd = 1.0f / sqrtf(block_sum(s, red) / (float)D + eps);
-        for (int d = threadIdx.x; d < D; d += kBlock) {
-            const float h = (to_f32(xr[d]) - mean) * rstd;
-            const float v = fmaf(h, w ? to_f32(w[d]) : 1.0f, b ? to_f32(b[d]) : 0.0f);
-            y[r * D + d] = from_f32<T>(drop_one(v, r * D + d, drop, key));
+        row_sum(s);
+        const float rstd = 1.0f / sqrtf(fmaf(s, inv, eps));
+        for (int d = threadIdx.x; d < D; d += kLong) {
+            float v[1] = {fmaf((to_f32(xr[d]) - mean) * rstd, w ? to_f32(w[d]) : 1.0f, b ? to_f32(b[d]) : 0.0f)};
+            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
+            y[r * D + d] = from_f32<T>(v[0]);
         }
         if (stats && threadIdx.x == 0) {
             stats[2 * r] = mean;
@@ -54,58 +351,63 @@ __global__ __launch_bounds__(kBlock) void k_norm_fwd(const T* __restrict__ x, in
     }
 }
 
-// d x, one workgroup per row.
 template <class T, class W>
-__global__ __launch_bounds__(kBlock) void k_norm_bwd_x(const T* __restrict__ gy, const T* __restrict__ x,
-                                                       int64_t stride, const W* __restrict__ w,
-                                                       const float* __restrict__ stats, int64_t rows, int D,
-                                                       Dropout drop, T* __restrict__ gx) {
-    __shared__ float red[kBlock / kWave];
-    const PhiloxKey key = philox_key(drop);
+__global__ __launch_bounds__(kLong) void k_norm_bwd_x_long(const T* __restrict__ gy, const T* __restrict__ x,
+                                                           int64_t stride, const W* __restrict__ w,
+                                                           const float* __restrict__ stats, int64_t rows, int D,
+                                                           Dropout drop_, T* __restrict__ gx) {
+    __shared__ float red[2][2][kLong / kWave];
+    RowSum<kLong> row_sum{red, 0};
+    const PhiloxKey key = philox_key(drop_);
+    const float inv = 1.0f / (float)D;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float mean = stats[2 * r], rstd = stats[2 * r + 1];
+        const auto at = [&](int d) {
+            float v[1] = {to_f32(gy[r * D + d])};
+            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
+            return v[0] * (w ? to_f32(w[d]) : 1.0f);
+        };
         float s0 = 0.0f, s1 = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kBlock) {
-            const float g = drop_one(to_f32(gy[r * D + d]), r * D + d, drop, key) * (w ? to_f32(w[d]) : 1.0f);
+        for (int d = threadIdx.x; d < D; d += kLong) {
+            const float g = at(d);
             s0 += g;
             s1 = fmaf(g, (to_f32(x[r * stride + d]) - mean) * rstd, s1);
         }
-        s0 = block_sum(s0, red) / (float)D;
-        s1 = block_sum(s1, red) / (float)D;
-        for (int d = threadIdx.x; d < D; d += kBlock) {
-            const float g = drop_one(to_f32(gy[r * D + d]), r * D + d, drop, key) * (w ? to_f32(w[d]) : 1.0f);
+        row_sum(s0, s1);
+        s0 *= inv;
+        s1 *= inv;
+        for (int d = threadIdx.x; d < D; d += kLong) {
             const float h = (to_f32(x[r * stride + d]) - mean) * rstd;
-            gx[r * D + d] = from_f32<T>(rstd * (g - s0 - h * s1));
+            gx[r * D + d] = from_f32<T>(rstd * (at(d) - fmaf(h, s1, s0)));
         }
     }
 }
 
-// d weight, d bias: a workgroup owns 64 columns, its four waves every fourth row.
-template <class T, class W>
-__global__ __launch_bounds__(kBlock) void k_norm_bwd_w(const T* __restrict__ gy, const T* __restrict__ x,
-                                                       int64_t stride, const float* __restrict__ stats, int64_t rows,
-                                                       int D, Dropout drop, W* __restrict__ gw, W* __restrict__ gb) {
+// part [gridDim.y][2][D]: workgroup (c, p) owns 64 columns and every gridDim.y-th group of four rows, a wave each.
+template <class T>
+__global__ __launch_bounds__(kBlock) void k_norm_bwd_w_long(const T* __restrict__ gy, const T* __restrict__ x,
+                                                            int64_t stride, const float* __restrict__ stats,
+                                                            int64_t rows, int D, Dropout drop_,
+                                                            float* __restrict__ part) {
     __shared__ float red[2][kBlock];
-    const PhiloxKey key = philox_key(drop);
+    const PhiloxKey key = philox_key(drop_);
     const int d = blockIdx.x * kWave + (threadIdx.x & (kWave - 1)), wave = threadIdx.x / kWave;
     float s0 = 0.0f, s1 = 0.0f;
     if (d < D)
-        for (int64_t r = wave; r < rows; r += kBlock / kWave) {
-            const float g = drop_one(to_f32(gy[r * D + d]), r * D + d, drop, key);
-            s0 += g;
-            s1 = fmaf(g, (to_f32(x[r * stride + d]) - stats[2 * r]) * stats[2 * r + 1], s1);
+        for (int64_t r = (int64_t)blockIdx.y * (kBlock / kWave) + wave; r < rows; r += (int64_t)gridDim.y * (kBlock / kWave)) {
+            float v[1] = {to_f32(gy[r * D + d])};
+            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
+            s0 += v[0];
+            s1 = fmaf(v[0], (to_f32(x[r * stride + d]) - stats[2 * r]) * stats[2 * r + 1], s1);
         }
-    red[0][threadIdx.x] = s0;
-    red[1][threadIdx.x] = s1;
+    red[0][threadIdx.x] = s1;
+    red[1][threadIdx.x] = s0;
     __syncthreads();
-    if (threadIdx.x < kWave && d < D) {
-        float t0 = 0.0f, t1 = 0.0f;
+    if (wave < 2 && d < D) {
+        const int at = threadIdx.x & (kWave - 1);
+        float t = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kBlock / kWave; ++k) {
-            t0 += red[0][k * kWave + threadIdx.x];
-            t1 += red[1][k * kWave + threadIdx.x];
-        }
-        if (gb) gb[d] = from_f32<W>(t0);
-        if (gw) gw[d] = from_f32<W>(t1);
+        for (int k = 0; k < kBlock / kWave; ++k) t += red[wave][k * kWave + at];
+        part[((size_t)blockIdx.y * 2 + wave) * D + d] = t;
     }
 }

@@ -483,7 +483,7 @@ int igs_embedding_backward(const void *grad_out, int dtype, const void *tokens, 
  * {block low, block high, offset low, offset high}, key {seed low, seed high}.  The seed is
  * *seed_device when that is not NULL (8 bytes of device memory read by the kernel, so that a replayed
  * graph sees what was written there since), else `seed`.  The same call on the upstream gradient is
- * the backward. */
+ * the backward.  0 <= count < 2^34. */
 int igs_dropout(const void *x, int dtype, int64_t count, int threshold, uint64_t seed,
                 const uint64_t *seed_device, uint64_t offset, void *y, igs_stream_t stream);
 
