@@ -104,6 +104,17 @@ def _rows(x: Tensor) -> Tuple[Tensor, int]:
     return x, sizes[-1] if step is None else step
 
 
+def _once(backward):
+    """`once_differentiable` without its bookkeeping where no graph of the backward is being recorded (grad
+    mode is off then): a training step of a small problem is bound by the host."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, grad):
+        return recorded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+
+    return run
+
+
 # --------------------------------------------------------------------------------------
 # embedding lookup
 # --------------------------------------------------------------------------------------
@@ -111,32 +122,35 @@ def _embedding_fwd(tokens: Tensor, weight: Tensor, scale: float) -> Tensor:
     vocab, D = weight.shape
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    if D > 1 and weight.stride(1) != 1:
-        weight = weight.contiguous()
-    dev = weight.device
+    step, column = weight.stride()
+    if column != 1 and D > 1:
+        weight, step = weight.contiguous(), D
+    dev, dtype = weight.device, weight.dtype
     with _on(dev):
-        out = torch.empty((*tokens.shape, D), dtype=weight.dtype, device=dev)
-        _lib.check(_lib.load().igs_embedding_forward(weight.data_ptr(), weight.stride(0), _DTYPES[weight.dtype], vocab,
-                                                     D, tokens.data_ptr(), _TOKENS[tokens.dtype], tokens.numel(), scale,
-                                                     out.data_ptr(), _stream(dev)), "igs_embedding_forward")
+        out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
+        rc = _lib.load().igs_embedding_forward(weight.data_ptr(), step, _DTYPES[dtype], vocab, D, tokens.data_ptr(),
+                                               _TOKENS[tokens.dtype], tokens.numel(), scale, out.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "igs_embedding_forward")
     return out
 
 
 def _embedding_bwd(grad: Tensor, tokens: Tensor, vocab: int, scale: float, padding_idx: int) -> Tensor:
-    D = grad.shape[-1]
     if not grad.is_contiguous():
         grad = grad.contiguous()
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    dev, code = grad.device, _DTYPES[grad.dtype]
-    nbytes = _lib.embedding_workspace_bytes(vocab, D, code, tokens.numel())
+    D, n, dtype, dev = grad.shape[-1], tokens.numel(), grad.dtype, grad.device
+    code = _DTYPES[dtype]
+    nbytes = _lib.embedding_workspace_bytes(vocab, D, code, n)
     with _on(dev):
-        out = torch.empty((vocab, D), dtype=grad.dtype, device=dev)
+        out = torch.empty((vocab, D), dtype=dtype, device=dev)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(_lib.load().igs_embedding_backward(grad.data_ptr(), code, tokens.data_ptr(), _TOKENS[tokens.dtype],
-                                                      tokens.numel(), vocab, D, scale, padding_idx, out.data_ptr(),
-                                                      None if ws is None else ws.data_ptr(), nbytes, _stream(dev)),
-                   "igs_embedding_backward")
+        rc = _lib.load().igs_embedding_backward(grad.data_ptr(), code, tokens.data_ptr(), _TOKENS[tokens.dtype], n, vocab,
+                                                D, scale, padding_idx, out.data_ptr(), ws.data_ptr() if nbytes else None,
+                                                nbytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "igs_embedding_backward")
     return out
 
 
@@ -148,7 +162,7 @@ class _Embedding(torch.autograd.Function):
         return _embedding_fwd(tokens, weight, scale)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         return None, _embedding_bwd(grad, ctx.saved_tensors[0], *ctx.args), None, None
 
@@ -232,48 +246,60 @@ def naive_embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, p
 # --------------------------------------------------------------------------------------
 def _norm_fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, threshold: int, seed: int,
               seed_tensor: Optional[Tensor], offset: int, want_stats: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    D = x.shape[-1]
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    step = D = shape[-1]
     rows = x.numel() // D
-    x, step = _rows(x)
-    dev, code = x.device, _DTYPES[x.dtype]
-    wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    if not x.is_contiguous():
+        x, step = _rows(x)
+    wdtype, pw, pb = dtype, None, None
+    if bias is not None:
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        wdtype, pb = bias.dtype, bias.data_ptr()
+    if weight is not None:
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        wdtype, pw = weight.dtype, weight.data_ptr()
     with _on(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = torch.empty(shape, dtype=dtype, device=dev)
         stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
-        _lib.check(_lib.load().igs_layer_norm_forward(
-            x.data_ptr(), step, code, None if weight is None else weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), _DTYPES[wdtype], rows, D, eps, threshold, seed,
+        rc = _lib.load().igs_layer_norm_forward(
+            x.data_ptr(), step, _DTYPES[dtype], pw, pb, _DTYPES[wdtype], rows, D, eps, threshold, seed,
             None if seed_tensor is None else seed_tensor.data_ptr(), offset, y.data_ptr(),
-            None if stats is None else stats.data_ptr(), _stream(dev)), "igs_layer_norm_forward")
+            stats.data_ptr() if want_stats else None, _stream(dev))
+    if rc:
+        _lib.check(rc, "igs_layer_norm_forward")
     return y, stats
 
 
 def _norm_bwd(grad: Tensor, x: Tensor, weight: Optional[Tensor], wdtype: torch.dtype, stats: Tensor, threshold: int,
               seed: int, seed_tensor: Optional[Tensor], offset: int, want_x: bool, want_w: bool, want_b: bool):
-    D = x.shape[-1]
-    rows = x.numel() // D
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    step = D = shape[-1]
+    rows = stats.shape[0]
     if not grad.is_contiguous():
         grad = grad.contiguous()
-    x, step = _rows(x)
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    dev, code, wcode = x.device, _DTYPES[x.dtype], _DTYPES[wdtype]
+    if not x.is_contiguous():
+        x, step = _rows(x)
+    pw = None
+    if weight is not None:
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        pw = weight.data_ptr()
+    code, wcode = _DTYPES[dtype], _DTYPES[wdtype]
     nbytes = _lib.layer_norm_workspace_bytes(rows, D, code, wcode) if want_w or want_b else 0
     with _on(dev):
-        gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
+        gx = torch.empty(shape, dtype=dtype, device=dev) if want_x else None
         gw = torch.empty(D, dtype=wdtype, device=dev) if want_w else None
         gb = torch.empty(D, dtype=wdtype, device=dev) if want_b else None
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(_lib.load().igs_layer_norm_backward(
-            grad.data_ptr(), x.data_ptr(), step, code, None if weight is None else weight.data_ptr(), wcode,
-            stats.data_ptr(), rows, D, threshold, seed, None if seed_tensor is None else seed_tensor.data_ptr(), offset,
-            None if gx is None else gx.data_ptr(), None if gw is None else gw.data_ptr(),
-            None if gb is None else gb.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(dev)),
-            "igs_layer_norm_backward")
+        rc = _lib.load().igs_layer_norm_backward(
+            grad.data_ptr(), x.data_ptr(), step, code, pw, wcode, stats.data_ptr(), rows, D, threshold, seed,
+            None if seed_tensor is None else seed_tensor.data_ptr(), offset, gx.data_ptr() if want_x else None,
+            gw.data_ptr() if want_w else None, gb.data_ptr() if want_b else None, ws.data_ptr() if nbytes else None,
+            nbytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "igs_layer_norm_backward")
     return gx, gw, gb
 
 
@@ -287,7 +313,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         x, weight, stats, seed_tensor = ctx.saved_tensors
         threshold, seed, offset = ctx.args
@@ -402,12 +428,14 @@ def naive_layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[
 def _dropout(x: Tensor, threshold: int, seed: int, seed_tensor: Optional[Tensor], offset: int) -> Tensor:
     if not x.is_contiguous():
         x = x.contiguous()
-    dev = x.device
+    dtype, dev = x.dtype, x.device
     with _on(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        _lib.check(_lib.load().igs_dropout(x.data_ptr(), _DTYPES[x.dtype], x.numel(), threshold, seed,
-                                           None if seed_tensor is None else seed_tensor.data_ptr(), offset,
-                                           y.data_ptr(), _stream(dev)), "igs_dropout")
+        y = torch.empty(x.shape, dtype=dtype, device=dev)
+        rc = _lib.load().igs_dropout(x.data_ptr(), _DTYPES[dtype], x.numel(), threshold, seed,
+                                     None if seed_tensor is None else seed_tensor.data_ptr(), offset, y.data_ptr(),
+                                     _stream(dev))
+    if rc:
+        _lib.check(rc, "igs_dropout")
     return y
 
 
@@ -419,7 +447,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, threshold, seed, seed_tensor, offset)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         threshold, seed, offset = ctx.args
         return _dropout(grad, threshold, seed, ctx.saved_tensors[0], offset), None, None, None, None
