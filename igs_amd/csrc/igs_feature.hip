@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <utility>
 
 #include "igs_hip.h"
 
@@ -53,6 +54,59 @@ int embedding_shape(int64_t vocab, int D, int64_t count) {
     return IGS_OK;
 }
 
+// What the dense gradient of a lookup is made of, a function of its sizes alone.
+struct EmbedPlan {
+    int passes, bits;        // of the sort: digits and their width
+    int tiles, tile;         // more than kSortOne tokens: tiles of so many keys
+    SumShape sum;
+    int64_t span;            // sorted places per group of k_embed_sum
+    int64_t padded;          // elements of a key or position array
+    size_t counts_at, partial_at, bytes;  // in the workspace, behind the arrays
+};
+
+#ifndef IGS_EMBED_SUM_WAVES
+#define IGS_EMBED_SUM_WAVES 8192
+#endif
+#ifndef IGS_EMBED_ZERO_BYTES
+#define IGS_EMBED_ZERO_BYTES (64 << 10)
+#endif
+
+EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
+    EmbedPlan p;
+    int total = 0;  // bits of the largest key, vocab itself
+    while (vocab >> total) ++total;
+    const bool one = n <= kSortOne;
+    const int most = one ? 8 : kSortBits;
+    p.passes = (total + most - 1) / most;
+    p.bits = (total + p.passes - 1) / p.passes;
+    p.tiles = p.tile = 0;
+    if (!one) {
+        p.tiles = (int)at_most(kSortTiles, ceil_div(n, 2 * kSortThreads));
+        p.tile = (int)(ceil_div(ceil_div(n, p.tiles), kSortThreads) * kSortThreads);
+        p.tiles = (int)ceil_div(n, p.tile);
+    }
+    const int V = D < 16 / dtype_bytes(dtype) ? 1 : 16 / dtype_bytes(dtype);
+    SumShape& s = p.sum;
+    s.packs = (int)ceil_div(D, V);
+    s.lanes = 8;
+    while (s.lanes < s.packs && s.lanes < kWave) s.lanes *= 2;
+    s.slices = (int)ceil_div(s.packs, s.lanes);
+    // places per unit: short enough for so many waves on the device, eight (one group of loads) at least
+    const int64_t waves = ceil_div(n, 1) * s.slices * s.lanes / kWave;
+    const int64_t len = ceil_div(ceil_div(waves, IGS_EMBED_SUM_WAVES), kUnroll) * kUnroll;
+    s.len = (int)(len < kUnroll ? kUnroll : len);
+    p.span = (int64_t)(kSumThreads / s.lanes) * s.len;
+    s.groups = (int)ceil_div(n, p.span);
+    const int64_t fit = IGS_EMBED_ZERO_BYTES / ((int64_t)D * dtype_bytes(dtype));
+    s.zero_rows = (int)(fit < 1 ? 1 : at_most(fit, kSumThreads));
+    p.padded = ceil_div(n, kUnroll) * kUnroll + kUnroll;
+    const size_t arrays = (size_t)p.padded * sizeof(int) * (one ? 2 : 4);
+    p.counts_at = (arrays + 15) & ~(size_t)15;
+    p.partial_at = (p.counts_at + ((size_t)p.tiles << p.bits) * sizeof(int) + 15) & ~(size_t)15;
+    p.bytes = p.partial_at + (s.groups > 1 ? (size_t)s.groups * 2 * D * sizeof(float) : 0);
+    return p;
+}
+
 int embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding_plan_t* p) {
     if (!p) return IGS_ERR_NULL_POINTER;
     if (!dtype_ok(dtype)) return IGS_ERR_BAD_DTYPE;
@@ -62,7 +116,7 @@ int embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding
     p->count = count;
     p->D = D;
     p->reserved = 0;
-    p->ws_bytes = 0;
+    p->ws_bytes = count ? make_embed_plan(vocab, D, dtype, count).bytes : 0;
     return IGS_OK;
 }
 
@@ -158,11 +212,49 @@ int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, c
     return launch_status();
 }
 
+template <class T, int V>
+void launch_embed_sum(const T* grad, const int* keys, const int* pos, int64_t n, int64_t vocab, int D, float scale,
+                      const EmbedPlan& p, float* partial, T* out, hipStream_t st) {
+    const SumShape& s = p.sum;
+    const int64_t work = (int64_t)s.groups * s.slices, zeroing = ceil_div(vocab, s.zero_rows);
+    hipLaunchKernelGGL((k_embed_sum<T, V>), dim3(work + zeroing), dim3(kSumThreads), 0, st, grad, keys, pos, n, vocab, D,
+                       scale, s, partial, out);
+    if (s.groups > 1)
+        hipLaunchKernelGGL((k_embed_join<T, V>), dim3(work), dim3(kSumThreads), 0, st, keys, n, vocab, D, scale, s, p.span,
+                           (const float*)partial, out);
+}
+
 template <class T, class I>
-int launch_embed_bwd(const void* grad, const void* tokens, int64_t count, int64_t vocab, int D, float scale,
-                     int64_t padding, void* out, hipStream_t st) {
-    hipLaunchKernelGGL((k_embed_bwd<T, I>), dim3(at_most(vocab, 1 << 20)), dim3(kBlock), 0, st, (const T*)grad,
-                       (const I*)tokens, count, vocab, D, scale, padding, (T*)out);
+int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vocab, int D, float scale,
+                     int64_t padding, void* out, void* ws, hipStream_t st) {
+    EmbedPlan p = make_embed_plan(vocab, D, sizeof(T) == 4 ? IGS_F32 : IGS_F16, n);
+    int *keys = (int*)ws, *pos = keys + p.padded;
+    float* partial = (float*)((char*)ws + p.partial_at);
+    if (n == 0) {
+        keys = pos = nullptr;  // nothing is read: every row is zeroed
+    } else if (!p.tiles) {
+        hipLaunchKernelGGL((k_sort_one<I>), dim3(1), dim3(kSortThreads), 0, st, (const I*)tokens, (int)n, vocab, padding,
+                           p.passes, p.bits, keys, pos);
+    } else {
+        int *other_keys = pos + p.padded, *other_pos = other_keys + p.padded;
+        int* counts = (int*)((char*)ws + p.counts_at);
+        SortSource<I> src{(const I*)tokens, nullptr, nullptr, vocab, padding};
+        for (int k = 0; k < p.passes; ++k) {
+            hipLaunchKernelGGL((k_sort_count<I>), dim3(p.tiles), dim3(kSortThreads), 0, st, src, n, p.tile, k * p.bits,
+                               p.bits, counts);
+            hipLaunchKernelGGL((k_sort_place<I>), dim3(p.tiles), dim3(kSortThreads), 0, st, src, n, p.tile, k * p.bits,
+                               p.bits, (const int*)counts, keys, pos);
+            src = SortSource<I>{nullptr, keys, pos, vocab, padding};
+            std::swap(keys, other_keys);
+            std::swap(pos, other_pos);
+        }
+        keys = other_keys;  // where the last pass wrote
+        pos = other_pos;
+    }
+    if (D < kVec<T>)
+        launch_embed_sum<T, 1>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, (T*)out, st);
+    else
+        launch_embed_sum<T, kVec<T>>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, (T*)out, st);
     return launch_status();
 }
 
@@ -291,7 +383,7 @@ int igs_embedding_backward(const void* grad_out, int dtype, const void* tokens, 
         !aligned_to(tokens, token_bytes))
         return IGS_ERR_ALIGNMENT;
     return IGS_BY_TOKENS(launch_embed_bwd, dtype, token_bytes, grad_out, tokens, count, vocab, D, scale, padding_idx,
-                         grad_weight, (hipStream_t)stream);
+                         grad_weight, ws, (hipStream_t)stream);
 }
 
 int igs_dropout(const void* x, int dtype, int64_t count, int threshold, uint64_t seed, const uint64_t* seed_device,
