@@ -197,21 +197,5 @@ def koleo_plan(B: int, N: int, D: int) -> KoleoPlan:
     return p
 
 
-@functools.lru_cache(maxsize=256)
-def embedding_workspace_bytes(vocab: int, D: int, dtype: int, count: int) -> int:
-    """Scratch of the lookup's dense gradient (pure host arithmetic in the library; cached)."""
-    p = EmbeddingPlan()
-    check(load().igs_embedding_plan(vocab, D, dtype, count, ctypes.byref(p)), "igs_embedding_plan")
-    return p.ws_bytes
-
-
-@functools.lru_cache(maxsize=256)
-def layer_norm_workspace_bytes(rows: int, D: int, dtype: int, wdtype: int) -> int:
-    """Scratch of the norm's backward (pure host arithmetic in the library; cached)."""
-    p = LayerNormPlan()
-    check(load().igs_layer_norm_plan(rows, D, dtype, wdtype, ctypes.byref(p)), "igs_layer_norm_plan")
-    return p.ws_bytes
-
-
 def strides6(sx, sy):
     return (c_int64 * 6)(*sx, *sy)

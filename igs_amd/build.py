@@ -1,4 +1,5 @@
-"""Builds igs_amd/libigs_hip.so (the C-ABI shared library) with hipcc for gfx950.
+"""Builds igs_amd/libigs_hip.so (the C-ABI shared library) with hipcc for gfx950, and igs_amd/_igs_torch.so
+(host code: the feature operators' autograd nodes around that library) with g++ against the installed torch.
 
 Usage: python -m igs_amd.build            (from the repository root)
 hipcc cross-compiles without a GPU; the built library sits in-tree next to this file.
@@ -13,6 +14,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SOURCES = [os.path.join(PKG, "csrc", f) for f in ("igs_gs2d.hip", "igs_feature.hip")]
 LIB = os.path.join(PKG, "libigs_hip.so")
+TORCH_SOURCE = os.path.join(PKG, "csrc", "igs_torch.cpp")
+TORCH_LIB = os.path.join(PKG, "_igs_torch.so")
 
 # Packed-fp32 instruction selection is switched off for all device code.
 HIPCC_FLAGS = [
@@ -34,14 +37,39 @@ def build(verbose: bool = True, extra=()) -> str:
     cmd = [hipcc, *HIPCC_FLAGS, *extra, "-o", LIB, *SOURCES]
     if verbose:
         print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+    host = subprocess.Popen(torch_command(verbose))   # beside the device code
+    try:
+        subprocess.check_call(cmd)
+    finally:
+        rc = host.wait()
+    if rc:
+        raise subprocess.CalledProcessError(rc, host.args)
     return LIB
 
 
+def torch_command(verbose: bool = True):
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DNDEBUG",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-DTORCH_EXTENSION_NAME=_igs_torch", "-I", os.path.join(ROOT, "include")]
+    for path in [*cpp_extension.include_paths(), os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+                 sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", path]
+    cmd += [TORCH_SOURCE, "-o", TORCH_LIB, "-L", lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ldl"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    return cmd
+
+
 def is_stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
     csrc = os.path.join(PKG, "csrc")
     deps = [os.path.join(csrc, f) for f in os.listdir(csrc)] + [os.path.join(ROOT, "include", "igs_hip.h")]
     return any(os.path.getmtime(d) > t for d in deps)

@@ -10,8 +10,8 @@ operators that make such a feature out of token ids or of a trunk's output, forw
 `GaussianSplatting2D` calls them when it is built with `num_embeddings=`, `feature_norm=` or
 `feature_dropout=`.  fp32, fp16 and bf16; sums and norms are held in fp32 and every result is rounded
 once; gradients of weights are summed in a fixed order (bit-reproducible).  Eager callers go through
-`torch.autograd.Function`s; under `torch.compile` the same library calls are registered operators
-(`igs_amd::embedding_fwd` and its like).  There is no CPU path: tensors must live on the GPU.  The
+native autograd nodes (csrc/igs_torch.cpp) around the C ABI; under `torch.compile` the same library
+calls are registered operators (`igs_amd::embedding_fwd` and its like).  There is no CPU path: tensors must live on the GPU.  The
 `naive_*` functions are the plain torch expressions (any device), what the module's `fused=False`
 debug path uses.
 """
@@ -21,15 +21,13 @@ import math
 from typing import List, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._splat import _on, _stream
 
 Tensor = torch.Tensor
 
 _DTYPES = {torch.float32: _lib.IGS_F32, torch.float16: _lib.IGS_F16, torch.bfloat16: _lib.IGS_BF16}
-_TOKENS = {torch.int64: 8, torch.int32: 4}
+_TOKENS = (torch.int64, torch.int32)
 
 
 # --------------------------------------------------------------------------------------
@@ -84,92 +82,30 @@ def _seed(seed, offset, like: Tensor) -> Tuple[int, Optional[Tensor], int]:
     return seed, None, offset
 
 
-def _rows(x: Tensor) -> Tuple[Tensor, int]:
-    """(x or a contiguous copy, distance of its rows in elements): rows of the last axis are taken where
-    they are if they are dense and evenly spaced (slices of the last axis, expanded batches)."""
-    if x.is_contiguous():
-        return x, x.shape[-1]
-    sizes, strides = x.shape, x.stride()
-    if sizes[-1] != 1 and strides[-1] != 1:
-        return x.contiguous(), sizes[-1]
-    step = span = None
-    for n, s in zip(reversed(sizes[:-1]), reversed(strides[:-1])):
-        if n == 1:
-            continue
-        if span is None:
-            step = s
-        elif s != span:
-            return x.contiguous(), sizes[-1]
-        span = s * n
-    return x, sizes[-1] if step is None else step
+_torch_binding = None
 
 
-def _once(backward):
-    """`once_differentiable` without its bookkeeping where no graph of the backward is being recorded (grad
-    mode is off then): a training step of a small problem is bound by the host."""
-    recorded = once_differentiable(backward)
-
-    def run(ctx, grad):
-        return recorded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
-
-    return run
+def _native():
+    """The binding's module, on the library that _lib has loaded; raises if either is missing."""
+    global _torch_binding
+    if _torch_binding is None:
+        lib = _lib.load()
+        try:
+            from . import _igs_torch
+        except ImportError as e:
+            raise _lib.IGSLibraryError(f"igs_amd/_igs_torch.so cannot be loaded ({e}): build it first "
+                                       "(python -m igs_amd.build)") from e
+        _igs_torch.bind(lib._handle)
+        _torch_binding = _igs_torch
+    return _torch_binding
 
 
 # --------------------------------------------------------------------------------------
 # embedding lookup
 # --------------------------------------------------------------------------------------
-def _embedding_fwd(tokens: Tensor, weight: Tensor, scale: float) -> Tensor:
-    vocab, D = weight.shape
-    if not tokens.is_contiguous():
-        tokens = tokens.contiguous()
-    step, column = weight.stride()
-    if column != 1 and D > 1:
-        weight, step = weight.contiguous(), D
-    dev, dtype = weight.device, weight.dtype
-    with _on(dev):
-        out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
-        rc = _lib.load().igs_embedding_forward(weight.data_ptr(), step, _DTYPES[dtype], vocab, D, tokens.data_ptr(),
-                                               _TOKENS[tokens.dtype], tokens.numel(), scale, out.data_ptr(), _stream(dev))
-    if rc:
-        _lib.check(rc, "igs_embedding_forward")
-    return out
-
-
-def _embedding_bwd(grad: Tensor, tokens: Tensor, vocab: int, scale: float, padding_idx: int) -> Tensor:
-    if not grad.is_contiguous():
-        grad = grad.contiguous()
-    if not tokens.is_contiguous():
-        tokens = tokens.contiguous()
-    D, n, dtype, dev = grad.shape[-1], tokens.numel(), grad.dtype, grad.device
-    code = _DTYPES[dtype]
-    nbytes = _lib.embedding_workspace_bytes(vocab, D, code, n)
-    with _on(dev):
-        out = torch.empty((vocab, D), dtype=dtype, device=dev)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        rc = _lib.load().igs_embedding_backward(grad.data_ptr(), code, tokens.data_ptr(), _TOKENS[tokens.dtype], n, vocab,
-                                                D, scale, padding_idx, out.data_ptr(), ws.data_ptr() if nbytes else None,
-                                                nbytes, _stream(dev))
-    if rc:
-        _lib.check(rc, "igs_embedding_backward")
-    return out
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx):
-        ctx.save_for_backward(tokens)
-        ctx.args = (weight.shape[0], scale, padding_idx)
-        return _embedding_fwd(tokens, weight, scale)
-
-    @staticmethod
-    @_once
-    def backward(ctx, grad):
-        return None, _embedding_bwd(grad, ctx.saved_tensors[0], *ctx.args), None, None
-
-
 @torch.library.custom_op("igs_amd::embedding_fwd", mutates_args=(), device_types="cuda")
 def embedding_fwd(tokens: Tensor, weight: Tensor, scale: float, padding_idx: int) -> Tensor:
-    return _embedding_fwd(tokens, weight, scale)
+    return _native().embedding_fwd(tokens, weight, scale)
 
 
 @embedding_fwd.register_fake
@@ -179,7 +115,7 @@ def _(tokens, weight, scale, padding_idx):
 
 @torch.library.custom_op("igs_amd::embedding_bwd", mutates_args=(), device_types="cuda")
 def embedding_bwd(grad: Tensor, tokens: Tensor, vocab: int, scale: float, padding_idx: int) -> Tensor:
-    return _embedding_bwd(grad, tokens, vocab, scale, padding_idx)
+    return _native().embedding_bwd(grad, tokens, vocab, scale, padding_idx)
 
 
 @embedding_bwd.register_fake
@@ -227,9 +163,7 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
     if torch.compiler.is_compiling():
         return torch.ops.igs_amd.embedding_fwd(tokens, weight, scale, padding_idx)
     _on_gpu(weight, tokens)
-    if weight.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(tokens, weight, scale, padding_idx)
-    return _embedding_fwd(tokens, weight.detach(), scale)
+    return (_torch_binding or _native()).embedding(tokens, weight, scale, padding_idx)
 
 
 def naive_embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
@@ -244,90 +178,11 @@ def naive_embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, p
 # --------------------------------------------------------------------------------------
 # layer norm (with dropout of its result)
 # --------------------------------------------------------------------------------------
-def _norm_fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, threshold: int, seed: int,
-              seed_tensor: Optional[Tensor], offset: int, want_stats: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    shape, dtype, dev = x.shape, x.dtype, x.device
-    step = D = shape[-1]
-    rows = x.numel() // D
-    if not x.is_contiguous():
-        x, step = _rows(x)
-    wdtype, pw, pb = dtype, None, None
-    if bias is not None:
-        if not bias.is_contiguous():
-            bias = bias.contiguous()
-        wdtype, pb = bias.dtype, bias.data_ptr()
-    if weight is not None:
-        if not weight.is_contiguous():
-            weight = weight.contiguous()
-        wdtype, pw = weight.dtype, weight.data_ptr()
-    with _on(dev):
-        y = torch.empty(shape, dtype=dtype, device=dev)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
-        rc = _lib.load().igs_layer_norm_forward(
-            x.data_ptr(), step, _DTYPES[dtype], pw, pb, _DTYPES[wdtype], rows, D, eps, threshold, seed,
-            None if seed_tensor is None else seed_tensor.data_ptr(), offset, y.data_ptr(),
-            stats.data_ptr() if want_stats else None, _stream(dev))
-    if rc:
-        _lib.check(rc, "igs_layer_norm_forward")
-    return y, stats
-
-
-def _norm_bwd(grad: Tensor, x: Tensor, weight: Optional[Tensor], wdtype: torch.dtype, stats: Tensor, threshold: int,
-              seed: int, seed_tensor: Optional[Tensor], offset: int, want_x: bool, want_w: bool, want_b: bool):
-    shape, dtype, dev = x.shape, x.dtype, x.device
-    step = D = shape[-1]
-    rows = stats.shape[0]
-    if not grad.is_contiguous():
-        grad = grad.contiguous()
-    if not x.is_contiguous():
-        x, step = _rows(x)
-    pw = None
-    if weight is not None:
-        if not weight.is_contiguous():
-            weight = weight.contiguous()
-        pw = weight.data_ptr()
-    code, wcode = _DTYPES[dtype], _DTYPES[wdtype]
-    nbytes = _lib.layer_norm_workspace_bytes(rows, D, code, wcode) if want_w or want_b else 0
-    with _on(dev):
-        gx = torch.empty(shape, dtype=dtype, device=dev) if want_x else None
-        gw = torch.empty(D, dtype=wdtype, device=dev) if want_w else None
-        gb = torch.empty(D, dtype=wdtype, device=dev) if want_b else None
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        rc = _lib.load().igs_layer_norm_backward(
-            grad.data_ptr(), x.data_ptr(), step, code, pw, wcode, stats.data_ptr(), rows, D, threshold, seed,
-            None if seed_tensor is None else seed_tensor.data_ptr(), offset, gx.data_ptr() if want_x else None,
-            gw.data_ptr() if want_w else None, gb.data_ptr() if want_b else None, ws.data_ptr() if nbytes else None,
-            nbytes, _stream(dev))
-    if rc:
-        _lib.check(rc, "igs_layer_norm_backward")
-    return gx, gw, gb
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, threshold, seed, seed_tensor, offset):
-        y, stats = _norm_fwd(x, weight, bias, eps, threshold, seed, seed_tensor, offset, True)
-        ctx.save_for_backward(x, weight, stats, seed_tensor)
-        ctx.args = (threshold, seed, offset)
-        ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, grad):
-        x, weight, stats, seed_tensor = ctx.saved_tensors
-        threshold, seed, offset = ctx.args
-        need = ctx.needs_input_grad
-        gx, gw, gb = _norm_bwd(grad, x, weight, ctx.wdtype, stats, threshold, seed, seed_tensor, offset, need[0],
-                               need[1], need[2])
-        return gx, gw, gb, None, None, None, None, None
-
-
 @torch.library.custom_op("igs_amd::layer_norm_fwd", mutates_args=(), device_types="cuda")
 def layer_norm_fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, threshold: int, seed: int,
                    seed_tensor: Optional[Tensor], offset: int) -> List[Tensor]:
     """[y, stats [rows, 2] (mean, 1 / standard deviation)]"""
-    return list(_norm_fwd(x, weight, bias, eps, threshold, seed, seed_tensor, offset, True))
+    return list(_native().layer_norm_fwd(x, weight, bias, eps, threshold, seed, seed_tensor, offset))
 
 
 @layer_norm_fwd.register_fake
@@ -339,10 +194,7 @@ def _(x, weight, bias, eps, threshold, seed, seed_tensor, offset):
 def layer_norm_bwd(grad: Tensor, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor,
                    threshold: int, seed: int, seed_tensor: Optional[Tensor], offset: int) -> List[Tensor]:
     """[grad_x, grad_weight (if weight), grad_bias (if bias)]"""
-    wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    g = _norm_bwd(grad, x, weight, wdtype, stats, threshold, seed, seed_tensor, offset, True, weight is not None,
-                  bias is not None)
-    return [t for t in g if t is not None]
+    return _native().layer_norm_bwd(grad, x, weight, bias, stats, threshold, seed, seed_tensor, offset)
 
 
 @layer_norm_bwd.register_fake
@@ -404,10 +256,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if torch.compiler.is_compiling():
         return torch.ops.igs_amd.layer_norm_fwd(x, weight, bias, eps, threshold, number, seed_tensor, offset)[0]
     _on_gpu(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps, threshold, number, seed_tensor, offset)
-    return _norm_fwd(x, weight, bias, eps, threshold, number, seed_tensor, offset, False)[0]
+    return (_torch_binding or _native()).layer_norm(x, weight, bias, eps, threshold, number, seed_tensor, offset)
 
 
 def naive_layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -425,37 +274,9 @@ def naive_layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[
 # --------------------------------------------------------------------------------------
 # dropout
 # --------------------------------------------------------------------------------------
-def _dropout(x: Tensor, threshold: int, seed: int, seed_tensor: Optional[Tensor], offset: int) -> Tensor:
-    if not x.is_contiguous():
-        x = x.contiguous()
-    dtype, dev = x.dtype, x.device
-    with _on(dev):
-        y = torch.empty(x.shape, dtype=dtype, device=dev)
-        rc = _lib.load().igs_dropout(x.data_ptr(), _DTYPES[dtype], x.numel(), threshold, seed,
-                                     None if seed_tensor is None else seed_tensor.data_ptr(), offset, y.data_ptr(),
-                                     _stream(dev))
-    if rc:
-        _lib.check(rc, "igs_dropout")
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, threshold, seed, seed_tensor, offset):
-        ctx.save_for_backward(seed_tensor)
-        ctx.args = (threshold, seed, offset)
-        return _dropout(x, threshold, seed, seed_tensor, offset)
-
-    @staticmethod
-    @_once
-    def backward(ctx, grad):
-        threshold, seed, offset = ctx.args
-        return _dropout(grad, threshold, seed, ctx.saved_tensors[0], offset), None, None, None, None
-
-
 @torch.library.custom_op("igs_amd::dropout", mutates_args=(), device_types="cuda")
 def dropout_op(x: Tensor, threshold: int, seed: int, seed_tensor: Optional[Tensor], offset: int) -> Tensor:
-    return _dropout(x, threshold, seed, seed_tensor, offset)
+    return _native().dropout_plain(x, threshold, seed, seed_tensor, offset)
 
 
 @dropout_op.register_fake
@@ -494,9 +315,7 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0) -> Tensor:
     if torch.compiler.is_compiling():
         return torch.ops.igs_amd.dropout(x, threshold, number, seed_tensor, offset)
     _on_gpu(x)
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Dropout.apply(x, threshold, number, seed_tensor, offset)
-    return _dropout(x, threshold, number, seed_tensor, offset)
+    return (_torch_binding or _native()).dropout(x, threshold, number, seed_tensor, offset)
 
 
 def _mul32(a: int, b: Tensor) -> Tuple[Tensor, Tensor]:

@@ -531,6 +531,30 @@ def test_a_seed_changed_before_the_backward_is_refused(igs, dev):
         y.sum().backward()
 
 
+def test_backward_twice_and_second_derivatives(igs, dev):
+    """A second backward without retain_graph and a derivative of the gradient raise; a graph recorded for something else
+    does not."""
+    x, w, t = torch.randn(5, 8, device=dev), torch.randn(8, device=dev), torch.tensor([1, 2, 2], device=dev)
+    table = torch.randn(4, 8, device=dev)
+    for f, leaf in ((lambda v: igs.embedding_lookup(t, v), table), (lambda v: igs.layer_norm(v, w), x),
+                    (lambda v: igs.layer_norm(x, v, dropout_p=0.2, seed=1), w), (lambda v: igs.dropout(v, 0.5, 1), x)):
+        v = leaf.clone().requires_grad_(True)
+        y = f(v)
+        up = torch.randn_like(y).requires_grad_(True)
+        (g,) = torch.autograd.grad(y, v, up, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
+        y = f(v)
+        (h,) = torch.autograd.grad(y, v, up.detach())
+        assert torch.equal(g.detach(), h)
+    y = igs.layer_norm(x.clone().requires_grad_(True), w)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    with torch.inference_mode():
+        assert torch.equal(igs.layer_norm(x, w), igs.layer_norm(x.clone(), w))
+
+
 def test_mixed_devices_raise(igs, dev):
     w, t, x = torch.randn(5, 4, device=dev), torch.tensor([1]), torch.randn(3, 4, device=dev)
     with pytest.raises(RuntimeError, match="same device"):
