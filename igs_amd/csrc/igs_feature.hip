@@ -67,8 +67,8 @@ struct EmbedPlan {
 #ifndef IGS_EMBED_SUM_WAVES
 #define IGS_EMBED_SUM_WAVES 8192
 #endif
-#ifndef IGS_EMBED_ZERO_BYTES
-#define IGS_EMBED_ZERO_BYTES (64 << 10)
+#ifndef IGS_EMBED_FILL_BYTES
+#define IGS_EMBED_FILL_BYTES (64 << 10)  // per filling workgroup
 #endif
 
 EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
@@ -87,19 +87,17 @@ EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
     }
     const int V = D < 16 / dtype_bytes(dtype) ? 1 : 16 / dtype_bytes(dtype);
     SumShape& s = p.sum;
-    s.packs = (int)ceil_div(D, V);
+    const int64_t packs = ceil_div(D, V);
     s.lanes = 8;
-    while (s.lanes < s.packs && s.lanes < kWave) s.lanes *= 2;
-    s.slices = (int)ceil_div(s.packs, s.lanes);
+    while (s.lanes < packs && s.lanes < kWave) s.lanes *= 2;
+    s.slices = (int)ceil_div(packs, s.lanes);
     // places per unit: short enough for so many waves on the device, eight (one group of loads) at least
-    const int64_t waves = ceil_div(n, 1) * s.slices * s.lanes / kWave;
+    const int64_t waves = n * s.slices * s.lanes / kWave;
     const int64_t len = ceil_div(ceil_div(waves, IGS_EMBED_SUM_WAVES), kUnroll) * kUnroll;
     s.len = (int)(len < kUnroll ? kUnroll : len);
     p.span = (int64_t)(kSumThreads / s.lanes) * s.len;
     s.groups = (int)ceil_div(n, p.span);
-    const int64_t fit = IGS_EMBED_ZERO_BYTES / ((int64_t)D * dtype_bytes(dtype));
-    s.zero_rows = (int)(fit < 1 ? 1 : at_most(fit, kSumThreads));
-    p.padded = ceil_div(n, kUnroll) * kUnroll + kUnroll;
+    p.padded = ceil_div(n, 4) * 4;
     const size_t arrays = (size_t)p.padded * sizeof(int) * (one ? 2 : 4);
     p.counts_at = (arrays + 15) & ~(size_t)15;
     p.partial_at = (p.counts_at + ((size_t)p.tiles << p.bits) * sizeof(int) + 15) & ~(size_t)15;
@@ -142,8 +140,10 @@ int device_cus() {
 }
 
 // How a row of D elements is laid over threads: TPR threads of NV packs of V elements.  The smallest
-// arrangement that holds the row: 16 elements per thread at most (more would cost the backward its
-// occupancy: x, gy, h, d, w and the two sums of every element are in registers).
+// arrangement that holds the row: a wave of up to 16 elements per thread, a workgroup of 256 threads of up
+// to 32, one of 512 (24 or 32).  More elements cost the backward, which has x, gy, h, d, w and the two
+// sums of every element in registers, its occupancy; a workgroup of 1024 threads leaves a thread too few
+// registers for 16 (fp16 2053 x 8205, backward: 65 us there).
 struct NormShape {
     int tpr, nv;
     bool one, is_long;  // V = 1; no arrangement holds the row
@@ -152,14 +152,16 @@ struct NormShape {
 NormShape norm_layout(int D, int dtype) {
     const int V = 16 / dtype_bytes(dtype);
     if (D < V) return {8, 1, true, false};
-    const int packs = (int)ceil_div(D, V);
-    const int most = 16 / V;  // packs per thread
+    const int packs = (int)ceil_div(D, V), unit = 8 / V;  // packs of eight elements
     for (int tpr = 8; tpr <= kWave; tpr *= 2)
         if (packs <= tpr) return {tpr, 1, false, false};
-    for (int tpr = kWave; tpr <= 1024; tpr *= 4)
-        for (int nv = tpr == kWave ? 2 : most / 2; nv <= most; nv *= 2)
-            if (packs <= tpr * nv) return {tpr, nv, false, false};
-    return {1024, 0, false, true};
+    for (int nv = 2; nv <= 2 * unit; nv *= 2)
+        if (packs <= kWave * nv) return {kWave, nv, false, false};
+    for (int k = 1; k <= 4; ++k)
+        if (packs <= 256 * k * unit) return {256, k * unit, false, false};
+    for (int k = 3; k <= 4; ++k)
+        if (packs <= 512 * k * unit) return {512, k * unit, false, false};
+    return {kLong, 0, false, true};
 }
 
 inline int norm_rows_at_once(const NormShape& s) { return s.tpr > kBlock ? 1 : kBlock / s.tpr; }
@@ -173,7 +175,7 @@ inline int norm_rows_at_once(const NormShape& s) { return s.tpr > kBlock ? 1 : k
 // Workgroups of the norm kernels: resident at once where there are more rows than that.
 int64_t norm_groups(const NormShape& s, int64_t rows, int per_cu) {
     const int64_t all = ceil_div(rows, norm_rows_at_once(s));
-    return at_most(all, (int64_t)device_cus() * (s.tpr > kBlock ? (per_cu + 3) / 4 : per_cu));
+    return at_most(all, (int64_t)device_cus() * (s.tpr > kBlock ? (per_cu + 1) / 2 : per_cu));
 }
 
 int norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* p) {
@@ -202,13 +204,21 @@ int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, c
     const int packs = D < V ? D : (int)ceil_div(D, V);
     int lanes = 1;
     while (lanes < packs && lanes < kBlock) lanes *= 2;
-    const int64_t groups = at_most(ceil_div(count, kBlock / lanes), 1 << 20);
-    if (D < V)
-        hipLaunchKernelGGL((k_embed_fwd<T, I, 1>), dim3(groups), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
-                           (const I*)tokens, count, scale, lanes, (T*)out);
-    else
-        hipLaunchKernelGGL((k_embed_fwd<T, I, V>), dim3(groups), dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D,
-                           (const I*)tokens, count, scale, lanes, (T*)out);
+    const int per = kBlock / lanes;
+    // four tokens in flight per thread where that still leaves eight workgroups per compute unit
+    const bool four = ceil_div(count, 4 * per) >= 8 * (int64_t)device_cus();
+    const dim3 grid(ceil_div(count, four ? 4 * per : per));
+#define IGS_EMBED_FWD(VV, U)                                                                                    \
+    hipLaunchKernelGGL((k_embed_fwd<T, I, VV, U>), grid, dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D, \
+                       (const I*)tokens, count, scale, lanes, (T*)out)
+    if (D < V) {
+        if (four) IGS_EMBED_FWD(1, 4);
+        else IGS_EMBED_FWD(1, 1);
+    } else {
+        if (four) IGS_EMBED_FWD(V, 4);
+        else IGS_EMBED_FWD(V, 1);
+    }
+#undef IGS_EMBED_FWD
     return launch_status();
 }
 
@@ -216,34 +226,54 @@ template <class T, int V>
 void launch_embed_sum(const T* grad, const int* keys, const int* pos, int64_t n, int64_t vocab, int D, float scale,
                       const EmbedPlan& p, float* partial, T* out, hipStream_t st) {
     const SumShape& s = p.sum;
-    const int64_t work = (int64_t)s.groups * s.slices, zeroing = ceil_div(vocab, s.zero_rows);
-    hipLaunchKernelGGL((k_embed_sum<T, V>), dim3(work + zeroing), dim3(kSumThreads), 0, st, grad, keys, pos, n, vocab, D,
-                       scale, s, partial, out);
+    const dim3 grid((int64_t)s.groups * s.slices);
+    if (s.lanes == kWave)
+        hipLaunchKernelGGL((k_embed_sum<T, V, true>), grid, dim3(kSumThreads), 0, st, grad, keys, pos, n, vocab, D, scale,
+                           s, partial, out);
+    else
+        hipLaunchKernelGGL((k_embed_sum<T, V, false>), grid, dim3(kSumThreads), 0, st, grad, keys, pos, n, vocab, D, scale,
+                           s, partial, out);
     if (s.groups > 1)
-        hipLaunchKernelGGL((k_embed_join<T, V>), dim3(work), dim3(kSumThreads), 0, st, keys, n, vocab, D, scale, s, p.span,
+        hipLaunchKernelGGL((k_embed_join<T, V>), grid, dim3(kSumThreads), 0, st, keys, n, vocab, D, scale, s, p.span,
                            (const float*)partial, out);
 }
 
 template <class T, class I>
 int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vocab, int D, float scale,
-                     int64_t padding, void* out, void* ws, hipStream_t st) {
-    EmbedPlan p = make_embed_plan(vocab, D, sizeof(T) == 4 ? IGS_F32 : IGS_F16, n);
+                     int64_t padding, void* out_, void* ws, hipStream_t st) {
+    const EmbedPlan p = make_embed_plan(vocab, D, sizeof(T) == 4 ? IGS_F32 : IGS_F16, n);
+    T* out = (T*)out_;
+    const int64_t total = vocab * D;
+    // workgroups that fill `count` elements with zeros
+    const auto filling = [](int64_t count) {
+        return at_most(ceil_div(count * (int64_t)sizeof(T), IGS_EMBED_FILL_BYTES), 1 << 20);
+    };
+    if (n == 0) {
+        hipLaunchKernelGGL((k_fill<T>), dim3(filling(total)), dim3(kSortThreads), 0, st, out, total);
+        return launch_status();
+    }
     int *keys = (int*)ws, *pos = keys + p.padded;
     float* partial = (float*)((char*)ws + p.partial_at);
-    if (n == 0) {
-        keys = pos = nullptr;  // nothing is read: every row is zeroed
-    } else if (!p.tiles) {
-        hipLaunchKernelGGL((k_sort_one<I>), dim3(1), dim3(kSortThreads), 0, st, (const I*)tokens, (int)n, vocab, padding,
-                           p.passes, p.bits, keys, pos);
+    if (!p.tiles) {
+        hipLaunchKernelGGL((k_sort_one<T, I>), dim3(1 + filling(total)), dim3(kSortThreads), 0, st, (const I*)tokens, (int)n,
+                           vocab, padding, p.passes, p.bits, keys, pos, out, total);
     } else {
         int *other_keys = pos + p.padded, *other_pos = other_keys + p.padded;
         int* counts = (int*)((char*)ws + p.counts_at);
         SortSource<I> src{(const I*)tokens, nullptr, nullptr, vocab, padding};
+        // every launch of the sort fills its share of the rows
+        const int64_t share = ceil_div(ceil_div(total, 2 * p.passes), 16) * 16;
+        int64_t filled = 0;
+        const auto next = [&] { return at_most(share, total - filled); };
         for (int k = 0; k < p.passes; ++k) {
-            hipLaunchKernelGGL((k_sort_count<I>), dim3(p.tiles), dim3(kSortThreads), 0, st, src, n, p.tile, k * p.bits,
-                               p.bits, counts);
-            hipLaunchKernelGGL((k_sort_place<I>), dim3(p.tiles), dim3(kSortThreads), 0, st, src, n, p.tile, k * p.bits,
-                               p.bits, (const int*)counts, keys, pos);
+            int64_t c = next();
+            hipLaunchKernelGGL((k_sort_count<T, I>), dim3(p.tiles + filling(c)), dim3(kSortThreads), 0, st, src, n, p.tile,
+                               p.tiles, k * p.bits, p.bits, counts, out + filled, c);
+            filled += c;
+            c = next();
+            hipLaunchKernelGGL((k_sort_place<T, I>), dim3(p.tiles + filling(c)), dim3(kSortThreads), 0, st, src, n, p.tile,
+                               p.tiles, k * p.bits, p.bits, (const int*)counts, keys, pos, out + filled, c);
+            filled += c;
             src = SortSource<I>{nullptr, keys, pos, vocab, padding};
             std::swap(keys, other_keys);
             std::swap(pos, other_pos);
@@ -252,9 +282,9 @@ int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vo
         pos = other_pos;
     }
     if (D < kVec<T>)
-        launch_embed_sum<T, 1>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, (T*)out, st);
+        launch_embed_sum<T, 1>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, out, st);
     else
-        launch_embed_sum<T, kVec<T>>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, (T*)out, st);
+        launch_embed_sum<T, kVec<T>>((const T*)grad, keys, pos, n, vocab, D, scale, p, partial, out, st);
     return launch_status();
 }
 
@@ -273,24 +303,24 @@ struct NormLayout {
 };
 template <class T, class F>
 void norm_dispatch(const NormShape& s, F f) {
-    constexpr int V = kVec<T>, kMost = 16 / V;
+    constexpr int V = kVec<T>, U = 8 / V;  // packs of eight elements
     if (s.one) return f(NormLayout<8, 1, 1>());
-    if (s.nv == 1 && s.tpr <= kWave) {
+    if (s.tpr <= kWave) {
         if (s.tpr == 8) return f(NormLayout<8, 1, V>());
         if (s.tpr == 16) return f(NormLayout<16, 1, V>());
         if (s.tpr == 32) return f(NormLayout<32, 1, V>());
-        return f(NormLayout<64, 1, V>());
-    }
-    if (s.tpr == kWave) {
+        if (s.nv == 1) return f(NormLayout<64, 1, V>());
         if (s.nv == 2) return f(NormLayout<64, 2, V>());
-        return f(NormLayout<64, kMost, V>());
+        return f(NormLayout<64, 2 * U, V>());
     }
     if (s.tpr == 256) {
-        if (s.nv == kMost / 2) return f(NormLayout<256, kMost / 2, V>());
-        return f(NormLayout<256, kMost, V>());
+        if (s.nv == U) return f(NormLayout<256, U, V>());
+        if (s.nv == 2 * U) return f(NormLayout<256, 2 * U, V>());
+        if (s.nv == 3 * U) return f(NormLayout<256, 3 * U, V>());
+        return f(NormLayout<256, 4 * U, V>());
     }
-    if (s.nv == kMost / 2) return f(NormLayout<1024, kMost / 2, V>());
-    return f(NormLayout<1024, kMost, V>());
+    if (s.nv == 3 * U) return f(NormLayout<512, 3 * U, V>());
+    return f(NormLayout<512, 4 * U, V>());
 }
 
 template <class T, class W>
@@ -331,7 +361,7 @@ int launch_norm_bwd(const void* gy, const void* x, int64_t stride, const void* w
         });
     }
     if (sums)
-        hipLaunchKernelGGL((k_norm_reduce<W>), dim3(ceil_div(2 * D, kWave)), dim3(kWave * kReduceWaves), 0, st,
+        hipLaunchKernelGGL((k_norm_reduce<W>), dim3(ceil_div(2 * D, kReduceCols)), dim3(kWave * kReduceWaves), 0, st,
                            (const float*)part, partials, D, (W*)gw, (W*)gb);
     return launch_status();
 }

@@ -5,7 +5,7 @@
 //   gx = rstd (g - mean g - h mean(g h)),  gw = sum_rows d h,  gb = sum_rows d
 //
 // Bound by memory: a row is read once and stays in registers between its sums and its result.  TPR
-// threads share a row (8 to 64 lanes of a wave, or a workgroup of 256 or 1024 threads), NV packs of 16
+// threads share a row (8 to 64 lanes of a wave, or a workgroup of 256 or 512 threads), NV packs of 16
 // bytes each; the weights of a thread's columns stay in registers while its workgroup walks over the
 // rows, the next row's loads in flight.  The last pack of a row whose length is no multiple of the
 // pack is moved back to end with the row: its first elements are the neighbour's (computed twice, counted
@@ -286,23 +286,25 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restr
     }
 }
 
-// gw, gb = the column sums of part [P][2][D].  A workgroup owns 64 of the 2 D columns; each of its 16 waves adds every
-// sixteenth partial row.
-constexpr int kReduceWaves = 16;
+// gw, gb = the column sums of part [P][2][D].  A workgroup owns 16 of the 2 D columns; each quarter of its 16 waves adds
+// every 64th partial row.
+constexpr int kReduceWaves = 16, kReduceCols = 16;
 template <class W>
 __global__ __launch_bounds__(kWave* kReduceWaves) void k_norm_reduce(const float* __restrict__ part, int P, int D,
                                                                      W* __restrict__ gw, W* __restrict__ gb) {
-    __shared__ float red[kReduceWaves][kWave];
+    __shared__ float red[kReduceWaves][kReduceCols];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int col = blockIdx.x * kWave + lane;
+    const int64_t col = (int64_t)blockIdx.x * kReduceCols + (lane & (kReduceCols - 1));
     float s = 0.0f;
-    if (col < 2 * D) {
+    if (col < 2 * (int64_t)D) {
 #pragma unroll 8
-        for (int p = wave; p < P; p += kReduceWaves) s += part[(size_t)p * 2 * D + col];
+        for (int p = wave * 4 + lane / kReduceCols; p < P; p += 4 * kReduceWaves) s += part[(size_t)p * 2 * D + col];
     }
-    red[wave][lane] = s;
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (lane < kReduceCols) red[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && col < 2 * D) {
+    if (threadIdx.x < kReduceCols && col < 2 * (int64_t)D) {
         s = 0.0f;
 #pragma unroll
         for (int k = 0; k < kReduceWaves; ++k) s += red[k][lane];
