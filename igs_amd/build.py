@@ -9,10 +9,11 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
-SOURCES = [os.path.join(PKG, "csrc", f) for f in ("igs_gs2d.hip", "igs_feature.hip")]
+SOURCES = [os.path.join(PKG, "csrc", f) for f in ("igs_gs2d.hip", "igs_feature.hip", "igs_norm.hip")]
 LIB = os.path.join(PKG, "libigs_hip.so")
 TORCH_SOURCE = os.path.join(PKG, "csrc", "igs_torch.cpp")
 TORCH_LIB = os.path.join(PKG, "_igs_torch.so")
@@ -23,7 +24,6 @@ HIPCC_FLAGS = [
     "-std=c++17",
     "--offload-arch=gfx950",
     "-fPIC",
-    "-shared",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # matrix-core results land in ordinary VGPRs (the vector ALU reads them without a copy out of
     # the accumulation registers); only the diversity-loss kernel uses the matrix cores
@@ -33,21 +33,26 @@ HIPCC_FLAGS = [
 
 
 def build(verbose: bool = True, extra=()) -> str:
+    """Every unit by a compiler of its own, side by side, then the library."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, *HIPCC_FLAGS, *extra, "-o", LIB, *SOURCES]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    host = subprocess.Popen(torch_command(verbose))   # beside the device code
-    try:
-        subprocess.check_call(cmd)
-    finally:
-        rc = host.wait()
-    if rc:
-        raise subprocess.CalledProcessError(rc, host.args)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SOURCES]
+        cmds = [[hipcc, *HIPCC_FLAGS, *extra, "-c", s, "-o", o] for s, o in zip(SOURCES, objects)] + [torch_command()]
+        running = []
+        for cmd in cmds:
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            running.append(subprocess.Popen(cmd))
+        for p in [p for p in running if p.wait()]:
+            raise subprocess.CalledProcessError(p.returncode, p.args)
+        link = [hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-o", LIB, *objects]
+        if verbose:
+            print(" ".join(link), flush=True)
+        subprocess.check_call(link)
     return LIB
 
 
-def torch_command(verbose: bool = True):
+def torch_command():
     import sysconfig
 
     import torch
@@ -61,8 +66,6 @@ def torch_command(verbose: bool = True):
                  sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", path]
     cmd += [TORCH_SOURCE, "-o", TORCH_LIB, "-L", lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ldl"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
     return cmd
 
 

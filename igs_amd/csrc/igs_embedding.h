@@ -60,12 +60,22 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kSortPer = 4;      // keys per thread of the one-workgroup sort, at most
+#ifndef IGS_SORT_PER
+#define IGS_SORT_PER 8
+#endif
+constexpr int kSortPer = IGS_SORT_PER;  // keys per thread of the one-workgroup sort, at most
 constexpr int kSortOne = kSortPer * kSortThreads;
 constexpr int kSortBits = 9;     // of a digit, at most
+constexpr int kSortHeld = 4;     // keys per thread that a tile's workgroup keeps in registers
 constexpr int kSortTiles = 128;  // at most: a tile's workgroup adds up the counts of all tiles itself
-constexpr int kSumThreads = 512;
-constexpr int kUnroll = 8;       // rows in a group of loads
+#ifndef IGS_SUM_THREADS
+#define IGS_SUM_THREADS 512
+#endif
+constexpr int kSumThreads = IGS_SUM_THREADS;
+#ifndef IGS_SUM_UNROLL
+#define IGS_SUM_UNROLL 8
+#endif
+constexpr int kUnroll = IGS_SUM_UNROLL;  // rows in a group of loads
 
 template <class I>
 __device__ __forceinline__ int token_key(I t, int64_t vocab, int64_t padding) {
@@ -155,8 +165,7 @@ template <class T, class I>
 __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I* __restrict__ tokens, int n, int64_t vocab,
                                                            int64_t padding, int passes, int bits, int* __restrict__ keys,
                                                            int* __restrict__ pos, T* __restrict__ out, int64_t out_count) {
-    constexpr int kBins = 1 << 8;
-    __shared__ int count[kSortWaves * kBins], part[8], sk[kSortOne], sp[kSortOne];
+    __shared__ int count[kSortWaves << kSortBits], part[8], sk[kSortOne], sp[kSortOne];
     if (blockIdx.x > 0) return fill_zero(out, out_count, blockIdx.x - 1, gridDim.x - 1);
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), bins = 1 << bits;
     const int per = (n + kSortThreads - 1) / kSortThreads;  // a wave owns 64 per consecutive keys
@@ -171,19 +180,19 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I* __restrict__
         const int shift = p * bits;
         for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) count[i] = 0;
         __syncthreads();
+        int* own = count + wave * bins;
+        int off[kSortPer];  // among the wave's equal digits; the counters end as the wave's counts
 #pragma unroll
         for (int j = 0; j < kSortPer; ++j)
-            if (at[j] >= 0) atomicAdd(&count[wave * bins + ((key[j] >> shift) & (bins - 1))], 1);
+            if (j < per) off[j] = take_place(own, (key[j] >> shift) & (bins - 1), bits, at[j] >= 0);  // uniform
         __syncthreads();
         wave_places(count, nullptr, nullptr, part, bins);
 #pragma unroll
         for (int j = 0; j < kSortPer; ++j)
-            if (j < per) {  // uniform
-                const int to = take_place(count + wave * bins, (key[j] >> shift) & (bins - 1), bits, at[j] >= 0);
-                if (at[j] >= 0) {
-                    sk[to] = key[j];
-                    sp[to] = at[j];
-                }
+            if (at[j] >= 0) {
+                const int to = own[(key[j] >> shift) & (bins - 1)] + off[j];
+                sk[to] = key[j];
+                sp[to] = at[j];
             }
         __syncthreads();
 #pragma unroll
@@ -232,8 +241,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(SortSource<I> src, 
 
 // Every key of a tile to its place: behind the smaller digits of all tiles, the equal digits of earlier tiles and those
 // of the same tile before it.  A wave owns a contiguous sixteenth of the tile.  The two halves of the workgroup add up
-// the counts of every other tile.  The workgroups behind the tiles fill out.
-template <class T, class I>
+// the counts of every other tile.  kHeld: a wave's keys fit kSortHeld registers and are read once, before anything is
+// waited for.  The workgroups behind the tiles fill out.
+template <class T, class I, bool kHeld>
 __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortSource<I> src, int64_t n, int tile, int tiles, int shift,
                                                              int bits, const int* __restrict__ counts,
                                                              int* __restrict__ keys, int* __restrict__ pos,
@@ -243,6 +253,20 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortSource<I> src, 
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), bins = 1 << bits;
     const int64_t i0 = (int64_t)blockIdx.x * tile + (int64_t)wave * (tile / kSortWaves);
     const int64_t end = i0 + tile / kSortWaves, i1 = end < n ? end : n;
+    int key[kSortHeld], at[kSortHeld];
+    if (kHeld) {
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j) {
+            const int64_t i = i0 + j * kWave + lane;
+            at[j] = -1;
+            if (i < i1) {
+                key[j] = src.key(i);
+                at[j] = src.position(i);
+            } else {
+                key[j] = 0;
+            }
+        }
+    }
     for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) count[i] = 0;
     const int half = threadIdx.x >> kSortBits, d = threadIdx.x & ((1 << kSortBits) - 1);
     int sum = 0, earlier = 0;
@@ -265,16 +289,34 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortSource<I> src, 
         all[d] += all[(1 << kSortBits) + d];
         before[d] += before[(1 << kSortBits) + d];
     }
-    for (int64_t i = i0 + lane; i < i1; i += kWave) atomicAdd(&count[wave * bins + ((src.key(i) >> shift) & (bins - 1))], 1);
+    int* own = count + wave * bins;
+    int off[kSortHeld];  // among the wave's equal digits; the counters end as the wave's counts
+    if (kHeld) {
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j)
+            if (i0 + j * kWave < i1) off[j] = take_place(own, (key[j] >> shift) & (bins - 1), bits, at[j] >= 0);
+    } else {
+        for (int64_t i = i0 + lane; i < i1; i += kWave) atomicAdd(&own[(src.key(i) >> shift) & (bins - 1)], 1);
+    }
     __syncthreads();
     wave_places(count, before, all, part, bins);
-    for (int64_t i = i0; i < i1; i += kWave) {  // wave-uniform
-        const bool valid = i + lane < i1;
-        const int key = valid ? src.key(i + lane) : 0;
-        const int to = take_place(count + wave * bins, (key >> shift) & (bins - 1), bits, valid);
-        if (valid) {
-            keys[to] = key;
-            pos[to] = src.position(i + lane);
+    if (kHeld) {
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j)
+            if (at[j] >= 0) {
+                const int to = own[(key[j] >> shift) & (bins - 1)] + off[j];
+                keys[to] = key[j];
+                pos[to] = at[j];
+            }
+    } else {
+        for (int64_t i = i0; i < i1; i += kWave) {  // wave-uniform
+            const bool valid = i + lane < i1;
+            const int k = valid ? src.key(i + lane) : 0;
+            const int to = take_place(own, (k >> shift) & (bins - 1), bits, valid);
+            if (valid) {
+                keys[to] = k;
+                pos[to] = src.position(i + lane);
+            }
         }
     }
 }

@@ -1,10 +1,10 @@
-// igs_feature.hip -- the operators in front of the module's head (the features that
-// src/igs/gs2d.py:611-635 of the reference takes as given): embedding lookup with its dense gradient,
-// layer norm forward and backward, dropout from a counter-based generator.  Kernels in the included
-// headers, argument checks and launches here.
+// igs_feature.hip -- operators in front of the module's head (the features that src/igs/gs2d.py:611-635
+// of the reference takes as given): embedding lookup with its dense gradient, and dropout from a
+// counter-based generator.  (Layer norm: igs_norm.hip.)  Kernels in the included headers, argument checks
+// and launches here.
 //
-// All of them are bound by memory traffic (a few operations per element); the sums of gradients over
-// rows or repeated tokens have a fixed order, so results are bit-reproducible run to run.
+// Both are bound by memory traffic (a few operations per element); the sums of gradients of repeated tokens
+// have a fixed order, so results are bit-reproducible run to run.
 
 #include <hip/hip_runtime.h>
 
@@ -18,36 +18,10 @@
 
 namespace {
 #include "igs_feature_common.h"
+#include "igs_feature_host.h"
 
 #include "igs_dropout.h"
 #include "igs_embedding.h"
-#include "igs_layer_norm.h"
-
-constexpr int64_t kMaxCount = 0x7FFFFFFE;
-constexpr int kMaxRow = 1 << 20;
-
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline int64_t at_most(int64_t v, int64_t most) { return v < most ? v : most; }
-
-inline int launch_status() {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? IGS_OK : (int)e;
-}
-
-inline bool dtype_ok(int t) { return t == IGS_F32 || t == IGS_F16 || t == IGS_BF16; }
-inline int dtype_bytes(int t) { return t == IGS_F32 ? 4 : 2; }
-inline bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
-
-int make_dropout(int threshold, uint64_t seed, const uint64_t* seed_device, uint64_t offset, Dropout* d) {
-    if (threshold < 0 || threshold > 65536) return IGS_ERR_BAD_ARGUMENT;
-    if (!aligned_to(seed_device, 8)) return IGS_ERR_ALIGNMENT;
-    d->threshold = (uint32_t)threshold;
-    d->factor = threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.0f;
-    d->seed = seed;
-    d->offset = offset;
-    d->seed_device = seed_device;
-    return IGS_OK;
-}
 
 int embedding_shape(int64_t vocab, int D, int64_t count) {
     if (vocab < 1 || vocab > kMaxCount || D < 1 || D > kMaxRow || count < 0 || count > kMaxCount) return IGS_ERR_BAD_SHAPE;
@@ -65,7 +39,7 @@ struct EmbedPlan {
 };
 
 #ifndef IGS_EMBED_SUM_WAVES
-#define IGS_EMBED_SUM_WAVES 8192
+#define IGS_EMBED_SUM_WAVES 4096
 #endif
 #ifndef IGS_EMBED_FILL_BYTES
 #define IGS_EMBED_FILL_BYTES (64 << 10)  // per filling workgroup
@@ -76,8 +50,7 @@ EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
     int total = 0;  // bits of the largest key, vocab itself
     while (vocab >> total) ++total;
     const bool one = n <= kSortOne;
-    const int most = one ? 8 : kSortBits;
-    p.passes = (total + most - 1) / most;
+    p.passes = (total + kSortBits - 1) / kSortBits;
     p.bits = (total + p.passes - 1) / p.passes;
     p.tiles = p.tile = 0;
     if (!one) {
@@ -115,85 +88,6 @@ int embedding_plan(int64_t vocab, int D, int dtype, int64_t count, igs_embedding
     p->D = D;
     p->reserved = 0;
     p->ws_bytes = count ? make_embed_plan(vocab, D, dtype, count).bytes : 0;
-    return IGS_OK;
-}
-
-int norm_shape(int64_t rows, int D, int dtype, int wdtype) {
-    if (!dtype_ok(dtype) || (wdtype != dtype && wdtype != IGS_F32)) return IGS_ERR_BAD_DTYPE;
-    if (rows < 0 || rows > kMaxCount || D < 1 || D > kMaxRow) return IGS_ERR_BAD_SHAPE;
-    return IGS_OK;
-}
-
-// Compute units of the current device (of an MI355X where there is none: plans are made without a GPU too).
-int device_cus() {
-    static std::atomic<int> cached{0};
-    int cus = cached.load(std::memory_order_relaxed);
-    if (cus > 0) return cus;
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) {
-        (void)hipGetLastError();
-        return 256;
-    }
-    cached.store(cus, std::memory_order_relaxed);
-    return cus;
-}
-
-// How a row of D elements is laid over threads: TPR threads of NV packs of V elements.  The smallest
-// arrangement that holds the row: a wave of up to 16 elements per thread, a workgroup of 256 threads of up
-// to 32, one of 512 (24 or 32).  More elements cost the backward, which has x, gy, h, d, w and the two
-// sums of every element in registers, its occupancy; a workgroup of 1024 threads leaves a thread too few
-// registers for 16 (fp16 2053 x 8205, backward: 65 us there).
-struct NormShape {
-    int tpr, nv;
-    bool one, is_long;  // V = 1; no arrangement holds the row
-};
-
-NormShape norm_layout(int D, int dtype) {
-    const int V = 16 / dtype_bytes(dtype);
-    if (D < V) return {8, 1, true, false};
-    const int packs = (int)ceil_div(D, V), unit = 8 / V;  // packs of eight elements
-    for (int tpr = 8; tpr <= kWave; tpr *= 2)
-        if (packs <= tpr) return {tpr, 1, false, false};
-    for (int nv = 2; nv <= 2 * unit; nv *= 2)
-        if (packs <= kWave * nv) return {kWave, nv, false, false};
-    for (int k = 1; k <= 4; ++k)
-        if (packs <= 256 * k * unit) return {256, k * unit, false, false};
-    for (int k = 3; k <= 4; ++k)
-        if (packs <= 512 * k * unit) return {512, k * unit, false, false};
-    return {kLong, 0, false, true};
-}
-
-inline int norm_rows_at_once(const NormShape& s) { return s.tpr > kBlock ? 1 : kBlock / s.tpr; }
-
-#ifndef IGS_NORM_FWD_WGS
-#define IGS_NORM_FWD_WGS 8
-#endif
-#ifndef IGS_NORM_BWD_WGS
-#define IGS_NORM_BWD_WGS 4
-#endif
-// Workgroups of the norm kernels: resident at once where there are more rows than that.
-int64_t norm_groups(const NormShape& s, int64_t rows, int per_cu) {
-    const int64_t all = ceil_div(rows, norm_rows_at_once(s));
-    return at_most(all, (int64_t)device_cus() * (s.tpr > kBlock ? (per_cu + 1) / 2 : per_cu));
-}
-
-int norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* p) {
-    if (!p) return IGS_ERR_NULL_POINTER;
-    const int rc = norm_shape(rows, D, dtype, wdtype);
-    if (rc) return rc;
-    const NormShape s = norm_layout(D, dtype);
-    int64_t P;
-    if (s.is_long) {  // row groups so that there are eight workgroups per compute unit
-        P = ceil_div((int64_t)device_cus() * 8, ceil_div(D, kWave));
-        P = at_most(P, ceil_div(rows, kBlock / kWave));
-    } else {
-        P = norm_groups(s, rows, IGS_NORM_BWD_WGS);
-    }
-    p->rows = rows;
-    p->D = D;
-    p->partials = (int32_t)P;
-    p->ws_bytes = (uint64_t)P * 2 * D * sizeof(float);
     return IGS_OK;
 }
 
@@ -271,8 +165,12 @@ int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vo
                                p.tiles, k * p.bits, p.bits, counts, out + filled, c);
             filled += c;
             c = next();
-            hipLaunchKernelGGL((k_sort_place<T, I>), dim3(p.tiles + filling(c)), dim3(kSortThreads), 0, st, src, n, p.tile,
-                               p.tiles, k * p.bits, p.bits, (const int*)counts, keys, pos, out + filled, c);
+            if (p.tile <= kSortHeld * kSortThreads)
+                hipLaunchKernelGGL((k_sort_place<T, I, true>), dim3(p.tiles + filling(c)), dim3(kSortThreads), 0, st, src, n,
+                                   p.tile, p.tiles, k * p.bits, p.bits, (const int*)counts, keys, pos, out + filled, c);
+            else
+                hipLaunchKernelGGL((k_sort_place<T, I, false>), dim3(p.tiles + filling(c)), dim3(kSortThreads), 0, st, src, n,
+                                   p.tile, p.tiles, k * p.bits, p.bits, (const int*)counts, keys, pos, out + filled, c);
             filled += c;
             src = SortSource<I>{nullptr, keys, pos, vocab, padding};
             std::swap(keys, other_keys);
@@ -296,81 +194,6 @@ int launch_dropout(const void* x, int64_t count, const Dropout& d, void* y, hipS
     return launch_status();
 }
 
-// f(TPR, NV, V) as constants for the arrangement `s` of a row
-template <int TPR, int NV, int V>
-struct NormLayout {
-    static constexpr int tpr = TPR, nv = NV, v = V;
-};
-template <class T, class F>
-void norm_dispatch(const NormShape& s, F f) {
-    constexpr int V = kVec<T>, U = 8 / V;  // packs of eight elements
-    if (s.one) return f(NormLayout<8, 1, 1>());
-    if (s.tpr <= kWave) {
-        if (s.tpr == 8) return f(NormLayout<8, 1, V>());
-        if (s.tpr == 16) return f(NormLayout<16, 1, V>());
-        if (s.tpr == 32) return f(NormLayout<32, 1, V>());
-        if (s.nv == 1) return f(NormLayout<64, 1, V>());
-        if (s.nv == 2) return f(NormLayout<64, 2, V>());
-        return f(NormLayout<64, 2 * U, V>());
-    }
-    if (s.tpr == 256) {
-        if (s.nv == U) return f(NormLayout<256, U, V>());
-        if (s.nv == 2 * U) return f(NormLayout<256, 2 * U, V>());
-        if (s.nv == 3 * U) return f(NormLayout<256, 3 * U, V>());
-        return f(NormLayout<256, 4 * U, V>());
-    }
-    if (s.nv == 3 * U) return f(NormLayout<512, 3 * U, V>());
-    return f(NormLayout<512, 4 * U, V>());
-}
-
-template <class T, class W>
-int launch_norm_fwd(const void* x, int64_t stride, const void* w, const void* b, int64_t rows, int D, float eps,
-                    const Dropout& d, void* y, float* stats, hipStream_t st) {
-    const NormShape s = norm_layout(D, sizeof(T) == 4 ? IGS_F32 : IGS_F16);
-    if (s.is_long)
-        hipLaunchKernelGGL((k_norm_fwd_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)x, stride,
-                           (const W*)w, (const W*)b, rows, D, eps, d, (T*)y, stats);
-    else
-        norm_dispatch<T>(s, [&](auto l) {
-            using L = decltype(l);
-            hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v>), dim3(norm_groups(s, rows, IGS_NORM_FWD_WGS)),
-                               dim3(norm_threads(L::tpr)), 0, st, (const T*)x, stride, (const W*)w, (const W*)b, rows, D,
-                               eps, d, (T*)y, stats);
-        });
-    return launch_status();
-}
-
-template <class T, class W>
-int launch_norm_bwd(const void* gy, const void* x, int64_t stride, const void* w, const float* stats, int64_t rows,
-                    int D, const Dropout& d, int partials, void* gx, void* gw, void* gb, float* part, hipStream_t st) {
-    const NormShape s = norm_layout(D, sizeof(T) == 4 ? IGS_F32 : IGS_F16);
-    const bool sums = gw || gb;
-    if (rows && s.is_long) {
-        if (gx)
-            hipLaunchKernelGGL((k_norm_bwd_x_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)gy,
-                               (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx);
-        if (sums)
-            hipLaunchKernelGGL((k_norm_bwd_w_long<T>), dim3(ceil_div(D, kWave), partials), dim3(kBlock), 0, st,
-                               (const T*)gy, (const T*)x, stride, stats, rows, D, d, part);
-    } else if (rows && (gx || sums)) {
-        norm_dispatch<T>(s, [&](auto l) {
-            using L = decltype(l);
-            hipLaunchKernelGGL((k_norm_bwd<T, W, L::tpr, L::nv, L::v>), dim3(partials), dim3(norm_threads(L::tpr)), 0, st,
-                               (const T*)gy, (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx,
-                               sums ? part : (float*)nullptr);
-        });
-    }
-    if (sums)
-        hipLaunchKernelGGL((k_norm_reduce<W>), dim3(ceil_div(2 * D, kReduceCols)), dim3(kWave * kReduceWaves), 0, st,
-                           (const float*)part, partials, D, (W*)gw, (W*)gb);
-    return launch_status();
-}
-
-// f<T, W>(args...) of the pair of types (norm_shape has refused the others)
-#define IGS_BY_TYPES(f, dtype, wdtype, ...)                                                             \
-    ((dtype) == IGS_F32   ? f<float, float>(__VA_ARGS__)                                                \
-     : (dtype) == IGS_F16 ? ((wdtype) == IGS_F32 ? f<f16, float>(__VA_ARGS__) : f<f16, f16>(__VA_ARGS__)) \
-                          : ((wdtype) == IGS_F32 ? f<bf16, float>(__VA_ARGS__) : f<bf16, bf16>(__VA_ARGS__)))
 // f<T, I>(args...) of an element type and a token width
 #define IGS_BY_TOKENS(f, dtype, bytes, ...)                                                            \
     ((dtype) == IGS_F32   ? ((bytes) == 8 ? f<float, int64_t>(__VA_ARGS__) : f<float, int32_t>(__VA_ARGS__)) \
@@ -431,50 +254,5 @@ int igs_dropout(const void* x, int dtype, int64_t count, int threshold, uint64_t
     return dtype == IGS_F32   ? launch_dropout<float>(x, count, d, y, st)
            : dtype == IGS_F16 ? launch_dropout<f16>(x, count, d, y, st)
                               : launch_dropout<bf16>(x, count, d, y, st);
-}
-
-int igs_layer_norm_forward(const void* x, int64_t x_row_stride, int dtype, const void* weight, const void* bias,
-                           int wdtype, int64_t rows, int D, float eps, int threshold, uint64_t seed,
-                           const uint64_t* seed_device, uint64_t offset, void* y, float* stats, igs_stream_t stream) {
-    int rc = norm_shape(rows, D, dtype, wdtype);
-    if (rc) return rc;
-    if (!(eps >= 0.0f) || !isfinite(eps) || x_row_stride < 0) return IGS_ERR_BAD_ARGUMENT;
-    Dropout d;
-    rc = make_dropout(threshold, seed, seed_device, offset, &d);
-    if (rc) return rc;
-    if (rows == 0) return IGS_OK;
-    if (!x || !y) return IGS_ERR_NULL_POINTER;
-    const int e = dtype_bytes(dtype), we = dtype_bytes(wdtype);
-    if (!aligned_to(x, e) || !aligned_to(y, e) || !aligned_to(weight, we) || !aligned_to(bias, we) ||
-        !aligned_to(stats, 8))
-        return IGS_ERR_ALIGNMENT;
-    return IGS_BY_TYPES(launch_norm_fwd, dtype, wdtype, x, x_row_stride, weight, bias, rows, D, eps, d, y, stats,
-                        (hipStream_t)stream);
-}
-
-int igs_layer_norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t* plan) {
-    return norm_plan(rows, D, dtype, wdtype, plan);
-}
-
-int igs_layer_norm_backward(const void* grad_y, const void* x, int64_t x_row_stride, int dtype, const void* weight,
-                            int wdtype, const float* stats, int64_t rows, int D, int threshold, uint64_t seed,
-                            const uint64_t* seed_device, uint64_t offset, void* grad_x, void* grad_weight,
-                            void* grad_bias, void* ws, size_t ws_bytes, igs_stream_t stream) {
-    igs_layer_norm_plan_t p;
-    int rc = norm_plan(rows, D, dtype, wdtype, &p);
-    if (rc) return rc;
-    if (x_row_stride < 0) return IGS_ERR_BAD_ARGUMENT;
-    Dropout d;
-    rc = make_dropout(threshold, seed, seed_device, offset, &d);
-    if (rc) return rc;
-    if (rows && (!grad_y || !x || !stats)) return IGS_ERR_NULL_POINTER;
-    if (p.ws_bytes && !ws && (grad_weight || grad_bias)) return IGS_ERR_NULL_POINTER;
-    if (ws_bytes < p.ws_bytes && (grad_weight || grad_bias)) return IGS_ERR_WORKSPACE;
-    const int e = dtype_bytes(dtype), we = dtype_bytes(wdtype);
-    if (!aligned_to(grad_y, e) || !aligned_to(x, e) || !aligned_to(grad_x, e) || !aligned_to(weight, we) ||
-        !aligned_to(grad_weight, we) || !aligned_to(grad_bias, we) || !aligned_to(stats, 8) || !aligned_to(ws, 16))
-        return IGS_ERR_ALIGNMENT;
-    return IGS_BY_TYPES(launch_norm_bwd, dtype, wdtype, grad_y, x, x_row_stride, weight, stats, rows, D, d, p.partials,
-                        grad_x, grad_weight, grad_bias, (float*)ws, (hipStream_t)stream);
 }
 }  // extern "C"

@@ -36,7 +36,7 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& q) {
     *reinterpret_cast<Pack<T, V>*>(p) = q;
 }
 
-// Sums over the TPR lanes of a row within a wave (TPR = 8, 16, 32 or 64), the same bits in all of them.
+// Sums over the TPR lanes of a row within a wave (TPR = 4, 8, 16, 32 or 64), the same bits in all of them.
 // Every lane of the wave takes part.  Data-parallel moves inside 16 lanes; a whole wave's four sums
 // of 16 are read as scalars.
 template <int kCtrl>
@@ -45,10 +45,10 @@ __device__ __forceinline__ float dpp_add(float v) {
 }
 template <int TPR>
 __device__ __forceinline__ float lanes_sum(float v) {
-    static_assert(TPR == 8 || TPR == 16 || TPR == 32 || TPR == 64, "");
+    static_assert(TPR == 4 || TPR == 8 || TPR == 16 || TPR == 32 || TPR == 64, "");
     v = dpp_add<0xB1>(v);   // lane ^ 1
     v = dpp_add<0x4E>(v);   // lane ^ 2
-    v = dpp_add<0x141>(v);  // mirrored within 8
+    if (TPR >= 8) v = dpp_add<0x141>(v);   // mirrored within 8
     if (TPR >= 16) v = dpp_add<0x140>(v);  // mirrored within 16
     if (TPR == 32) v += __shfl_xor(v, 16);
     if (TPR == 64) {

@@ -316,35 +316,61 @@ __global__ __launch_bounds__(kWave* kReduceWaves) void k_norm_reduce(const float
     }
 }
 
-// ---- rows that do not fit a workgroup's registers: read again for every step -------------------------
+// ---- wide rows ------------------------------------------------------------------------------------------
 constexpr int kLong = 1024;
 
+// Rows that fit no workgroup's registers: read three times, the second and third time from the caches.
 template <class T, class W>
 __global__ __launch_bounds__(kLong) void k_norm_fwd_long(const T* __restrict__ x, int64_t stride,
                                                          const W* __restrict__ w, const W* __restrict__ b,
                                                          int64_t rows, int D, float eps, Dropout drop_,
                                                          T* __restrict__ y, float* __restrict__ stats) {
+    constexpr int V = kVec<T>;
     __shared__ float red[2][2][kLong / kWave];
     RowSum<kLong> row_sum{red, 0};
     const PhiloxKey key = philox_key(drop_);
     const float inv = 1.0f / (float)D;
+    const bool whole = D % 8 == 0;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + r * stride;
         float s = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kLong) s += to_f32(xr[d]);
+#pragma unroll 2
+        for (int col = threadIdx.x * V; col < D; col += kLong * V) {
+            const int start = col + V <= D ? col : D - V;
+            const Pack<T, V> q = load_pack<T, V>(xr + start);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += start + j >= col ? to_f32(q.v[j]) : 0.0f;
+        }
         row_sum(s);
         const float mean = s * inv;
         s = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kLong) {
-            const float c = to_f32(xr[d]) - mean;
-            s = fmaf(c, c, s);
+#pragma unroll 2
+        for (int col = threadIdx.x * V; col < D; col += kLong * V) {
+            const int start = col + V <= D ? col : D - V;
+            const Pack<T, V> q = load_pack<T, V>(xr + start);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float c = start + j >= col ? to_f32(q.v[j]) - mean : 0.0f;
+                s = fmaf(c, c, s);
+            }
         }
         row_sum(s);
         const float rstd = 1.0f / sqrtf(fmaf(s, inv, eps));
-        for (int d = threadIdx.x; d < D; d += kLong) {
-            float v[1] = {fmaf((to_f32(xr[d]) - mean) * rstd, w ? to_f32(w[d]) : 1.0f, b ? to_f32(b[d]) : 0.0f)};
-            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
-            y[r * D + d] = from_f32<T>(v[0]);
+#pragma unroll 2
+        for (int col = threadIdx.x * V; col < D; col += kLong * V) {
+            const int start = col + V <= D ? col : D - V;
+            Pack<T, V> q = load_pack<T, V>(xr + start);
+            Pack<W, V> pw, pb;
+            if (w) pw = load_pack<W, V>(w + start);
+            if (b) pb = load_pack<W, V>(b + start);
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                v[j] = fmaf((to_f32(q.v[j]) - mean) * rstd, w ? to_f32(pw.v[j]) : 1.0f, b ? to_f32(pb.v[j]) : 0.0f);
+            if (drop_.threshold) drop<V>(v, (uint64_t)r * D + start, whole, drop_, key);
+#pragma unroll
+            for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(v[j]);
+            store_pack<T, V>(y + r * D + start, q);
         }
         if (stats && threadIdx.x == 0) {
             stats[2 * r] = mean;
@@ -353,63 +379,130 @@ __global__ __launch_bounds__(kLong) void k_norm_fwd_long(const T* __restrict__ x
     }
 }
 
+// Backward of rows of more than 4096 elements, in two kernels.  Holding such a row's x, gy, weights and sums in one
+// workgroup's registers leaves one or two waves per SIMD and a partial row of 2 D sums from each workgroup (fp16
+// 2053 x 8205: 47 us); reading x and gy a second time, the better part of it from the last-level cache, costs less.
+// sums[r] = (mean g, mean (g h)) of row r.
 template <class T, class W>
-__global__ __launch_bounds__(kLong) void k_norm_bwd_x_long(const T* __restrict__ gy, const T* __restrict__ x,
-                                                           int64_t stride, const W* __restrict__ w,
-                                                           const float* __restrict__ stats, int64_t rows, int D,
-                                                           Dropout drop_, T* __restrict__ gx) {
-    __shared__ float red[2][2][kLong / kWave];
-    RowSum<kLong> row_sum{red, 0};
+__global__ __launch_bounds__(kBlock) void k_norm_bwd_sums(const T* __restrict__ gy, const T* __restrict__ x,
+                                                          int64_t stride, const W* __restrict__ w,
+                                                          const float* __restrict__ stats, int64_t rows, int D,
+                                                          Dropout drop_, float2* __restrict__ sums) {
+    constexpr int V = kVec<T>;
+    __shared__ float red[2][2][kBlock / kWave];
+    RowSum<kBlock> row_sum{red, 0};
     const PhiloxKey key = philox_key(drop_);
     const float inv = 1.0f / (float)D;
+    const bool whole = D % 8 == 0;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float mean = stats[2 * r], rstd = stats[2 * r + 1];
-        const auto at = [&](int d) {
-            float v[1] = {to_f32(gy[r * D + d])};
-            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
-            return v[0] * (w ? to_f32(w[d]) : 1.0f);
-        };
         float s0 = 0.0f, s1 = 0.0f;
-        for (int d = threadIdx.x; d < D; d += kLong) {
-            const float g = at(d);
-            s0 += g;
-            s1 = fmaf(g, (to_f32(x[r * stride + d]) - mean) * rstd, s1);
+#pragma unroll 4
+        for (int col = threadIdx.x * V; col < D; col += kBlock * V) {
+            const int start = col + V <= D ? col : D - V;
+            const Pack<T, V> qx = load_pack<T, V>(x + r * stride + start), qg = load_pack<T, V>(gy + r * D + start);
+            Pack<W, V> pw;
+            if (w) pw = load_pack<W, V>(w + start);
+            float d[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[j] = to_f32(qg.v[j]);
+            if (drop_.threshold) drop<V>(d, (uint64_t)r * D + start, whole, drop_, key);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float g = start + j >= col ? d[j] * (w ? to_f32(pw.v[j]) : 1.0f) : 0.0f;
+                s0 += g;
+                s1 = fmaf(g, (to_f32(qx.v[j]) - mean) * rstd, s1);
+            }
         }
         row_sum(s0, s1);
-        s0 *= inv;
-        s1 *= inv;
-        for (int d = threadIdx.x; d < D; d += kLong) {
-            const float h = (to_f32(x[r * stride + d]) - mean) * rstd;
-            gx[r * D + d] = from_f32<T>(rstd * (at(d) - fmaf(h, s1, s0)));
-        }
+        if (threadIdx.x == 0) sums[r] = make_float2(s0 * inv, s1 * inv);
     }
 }
 
-// part [gridDim.y][2][D]: workgroup (c, p) owns 64 columns and every gridDim.y-th group of four rows, a wave each.
-template <class T>
-__global__ __launch_bounds__(kBlock) void k_norm_bwd_w_long(const T* __restrict__ gy, const T* __restrict__ x,
-                                                            int64_t stride, const float* __restrict__ stats,
-                                                            int64_t rows, int D, Dropout drop_,
-                                                            float* __restrict__ part) {
-    __shared__ float red[2][kBlock];
+// Workgroup (slice, group) owns 64 packs of columns, a pack per lane, and walks with four waves over every
+// gridDim.y-th group of four rows, kRowsAhead of a wave's rows in flight.  part [gridDim.y][2][D].
+constexpr int kRowsAhead = 4;
+template <class T, class W>
+__global__ __launch_bounds__(kBlock) void k_norm_bwd_cols(const T* __restrict__ gy, const T* __restrict__ x,
+                                                          int64_t stride, const W* __restrict__ w,
+                                                          const float* __restrict__ stats,
+                                                          const float2* __restrict__ sums, int64_t rows, int D,
+                                                          Dropout drop_, T* __restrict__ gx, float* __restrict__ part) {
+    constexpr int V = kVec<T>, kWaves = kBlock / kWave;
+    __shared__ alignas(16) float red[kWaves - 1][2][kWave][V];
     const PhiloxKey key = philox_key(drop_);
-    const int d = blockIdx.x * kWave + (threadIdx.x & (kWave - 1)), wave = threadIdx.x / kWave;
-    float s0 = 0.0f, s1 = 0.0f;
-    if (d < D)
-        for (int64_t r = (int64_t)blockIdx.y * (kBlock / kWave) + wave; r < rows; r += (int64_t)gridDim.y * (kBlock / kWave)) {
-            float v[1] = {to_f32(gy[r * D + d])};
-            if (drop_.threshold) drop<1>(v, (uint64_t)r * D + d, false, drop_, key);
-            s0 += v[0];
-            s1 = fmaf(v[0], (to_f32(x[r * stride + d]) - stats[2 * r]) * stats[2 * r + 1], s1);
-        }
-    red[0][threadIdx.x] = s1;
-    red[1][threadIdx.x] = s0;
-    __syncthreads();
-    if (wave < 2 && d < D) {
-        const int at = threadIdx.x & (kWave - 1);
-        float t = 0.0f;
+    const bool whole = D % 8 == 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+    const int col = ((int)blockIdx.x * kWave + lane) * V;
+    const bool mine = col < D;
+    const int start = !mine ? 0 : col + V <= D ? col : D - V;
+    float wv[V], aw[V], ab[V];
+    Pack<W, V> pw;
+    if (w) pw = load_pack<W, V>(w + start);
 #pragma unroll
-        for (int k = 0; k < kBlock / kWave; ++k) t += red[wave][k * kWave + at];
-        part[((size_t)blockIdx.y * 2 + wave) * D + d] = t;
+    for (int j = 0; j < V; ++j) {
+        wv[j] = w ? to_f32(pw.v[j]) : 1.0f;
+        aw[j] = ab[j] = 0.0f;
+    }
+    const int64_t step = (int64_t)gridDim.y * kWaves;
+    for (int64_t r0 = (int64_t)blockIdx.y * kWaves + wave; r0 < rows; r0 += step * kRowsAhead) {
+        Pack<T, V> qx[kRowsAhead], qg[kRowsAhead];
+        float2 st[kRowsAhead], sm[kRowsAhead];
+#pragma unroll
+        for (int u = 0; u < kRowsAhead; ++u) {
+            const int64_t r = r0 + u * step < rows ? r0 + u * step : r0;
+            qx[u] = load_pack<T, V>(x + r * stride + start);
+            qg[u] = load_pack<T, V>(gy + r * D + start);
+            st[u] = reinterpret_cast<const float2*>(stats)[r];
+            if (gx) sm[u] = sums[r];
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsAhead; ++u) {
+            const int64_t r = r0 + u * step;
+            if (r >= rows) break;  // uniform
+            float d[V], h[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                d[j] = to_f32(qg[u].v[j]);
+                h[j] = (to_f32(qx[u].v[j]) - st[u].x) * st[u].y;
+            }
+            if (drop_.threshold) drop<V>(d, (uint64_t)r * D + start, whole, drop_, key);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                aw[j] = fmaf(d[j], h[j], aw[j]);
+                ab[j] += d[j];
+            }
+            if (gx && mine) {
+                Pack<T, V> q;
+#pragma unroll
+                for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(st[u].y * (d[j] * wv[j] - fmaf(h[j], sm[u].y, sm[u].x)));
+                store_pack<T, V>(gx + r * D + start, q);
+            }
+        }
+    }
+    if (!part) return;
+    if (wave > 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            red[wave - 1][0][lane][j] = aw[j];
+            red[wave - 1][1][lane][j] = ab[j];
+        }
+    }
+    __syncthreads();
+    if (wave == 0 && mine) {
+        float* out = part + (size_t)blockIdx.y * 2 * D + start;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float a = aw[j], c = ab[j];
+#pragma unroll
+            for (int k = 0; k < kWaves - 1; ++k) {
+                a += red[k][0][lane][j];
+                c += red[k][1][lane][j];
+            }
+            if (start + j >= col) {
+                out[j] = a;
+                out[D + j] = c;
+            }
+        }
     }
 }

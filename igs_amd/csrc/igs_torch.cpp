@@ -167,7 +167,6 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
     const int wcode = wtype == at::kFloat ? IGS_F32 : wtype == at::kHalf ? IGS_F16 : IGS_BF16;
     igs_layer_norm_plan_t plan;
     check(lib.layer_norm_plan(rows, width(D), code, wcode, &plan), "igs_layer_norm_plan");
-    if (!want_w && !want_b) plan.ws_bytes = 0;
     const Tensor ws = workspace(plan.ws_bytes, x);
     check(lib.layer_norm_backward(address(grad), address(x), step, code, address(weight), wcode,
                                   static_cast<const float*>(address(stats)), rows, width(D),
