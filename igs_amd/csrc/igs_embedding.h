@@ -54,6 +54,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
 //   k_embed_sum                 runs of equal keys added up; runs that cross a workgroup's border leave
 //                               partial rows
 //   k_embed_join                adds those
+//   k_embed_small               all of it, for few tokens
 // The sort waits on memory and keeps few compute units busy; the other workgroups of its launches fill the
 // table's gradient with zeros meanwhile, so that k_embed_sum writes the rows that tokens name and no more.
 // Every sum has a fixed order; the atomics are integer counters in LDS.
@@ -160,6 +161,51 @@ __global__ __launch_bounds__(kSortThreads) void k_fill(T* __restrict__ out, int6
     fill_zero(out, count, blockIdx.x, gridDim.x);
 }
 
+// The sort within one workgroup: up to kPer keys per thread, left sorted in sk and their positions in sp.  `count`:
+// kSortWaves << bits ints, `part` 8 ints of LDS.
+template <int kPer, class I>
+__device__ __forceinline__ void sort_here(const I* __restrict__ tokens, int n, int64_t vocab, int64_t padding, int passes,
+                                          int bits, int* count, int* part, int* sk, int* sp) {
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), bins = 1 << bits;
+    const int per = (n + kSortThreads - 1) / kSortThreads;  // a wave owns 64 per consecutive keys
+    int* own = count + wave * bins;
+    int key[kPer], at[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = (wave * per + j) * kWave + lane;
+        at[j] = j < per && i < n ? i : -1;
+        key[j] = at[j] >= 0 ? token_key(tokens[i], vocab, padding) : 0;
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * bits;
+        if (p > 0) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (at[j] >= 0) {
+                    const int i = (wave * per + j) * kWave + lane;
+                    key[j] = sk[i];
+                    at[j] = sp[i];
+                }
+        }
+        for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) count[i] = 0;
+        __syncthreads();
+        int off[kPer];  // among the wave's equal digits; the counters end as the wave's counts
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (j < per) off[j] = take_place(own, (key[j] >> shift) & (bins - 1), bits, at[j] >= 0);  // uniform
+        __syncthreads();
+        wave_places(count, nullptr, nullptr, part, bins);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (at[j] >= 0) {
+                const int to = own[(key[j] >> shift) & (bins - 1)] + off[j];
+                sk[to] = key[j];
+                sp[to] = at[j];
+            }
+        __syncthreads();
+    }
+}
+
 // keys, pos [n]: sorted keys and their places in `tokens`.  The workgroups behind the first fill out.
 template <class T, class I>
 __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I* __restrict__ tokens, int n, int64_t vocab,
@@ -167,50 +213,11 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I* __restrict__
                                                            int* __restrict__ pos, T* __restrict__ out, int64_t out_count) {
     __shared__ int count[kSortWaves << kSortBits], part[8], sk[kSortOne], sp[kSortOne];
     if (blockIdx.x > 0) return fill_zero(out, out_count, blockIdx.x - 1, gridDim.x - 1);
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), bins = 1 << bits;
-    const int per = (n + kSortThreads - 1) / kSortThreads;  // a wave owns 64 per consecutive keys
-    int key[kSortPer], at[kSortPer];
-#pragma unroll
-    for (int j = 0; j < kSortPer; ++j) {
-        const int i = (wave * per + j) * kWave + lane;
-        at[j] = j < per && i < n ? i : -1;
-        key[j] = at[j] >= 0 ? token_key(tokens[i], vocab, padding) : 0;
+    sort_here<kSortPer>(tokens, n, vocab, padding, passes, bits, count, part, sk, sp);
+    for (int i = threadIdx.x; i < n; i += kSortThreads) {
+        keys[i] = sk[i];
+        pos[i] = sp[i];
     }
-    for (int p = 0; p < passes; ++p) {
-        const int shift = p * bits;
-        for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) count[i] = 0;
-        __syncthreads();
-        int* own = count + wave * bins;
-        int off[kSortPer];  // among the wave's equal digits; the counters end as the wave's counts
-#pragma unroll
-        for (int j = 0; j < kSortPer; ++j)
-            if (j < per) off[j] = take_place(own, (key[j] >> shift) & (bins - 1), bits, at[j] >= 0);  // uniform
-        __syncthreads();
-        wave_places(count, nullptr, nullptr, part, bins);
-#pragma unroll
-        for (int j = 0; j < kSortPer; ++j)
-            if (at[j] >= 0) {
-                const int to = own[(key[j] >> shift) & (bins - 1)] + off[j];
-                sk[to] = key[j];
-                sp[to] = at[j];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kSortPer; ++j)
-            if (at[j] >= 0) {
-                const int i = (wave * per + j) * kWave + lane;
-                key[j] = sk[i];
-                at[j] = sp[i];
-            }
-        // (the barriers of the next pass stand between these reads and its writes)
-    }
-#pragma unroll
-    for (int j = 0; j < kSortPer; ++j)
-        if (at[j] >= 0) {
-            const int i = (wave * per + j) * kWave + lane;
-            keys[i] = key[j];
-            pos[i] = at[j];
-        }
 }
 
 // Where a pass of the sort finds its keys: in the tokens (first pass) or where the pass before left them.
@@ -339,16 +346,15 @@ __device__ __forceinline__ void write_row(T* __restrict__ out, int64_t row, int 
 // partial [groups][2][D]: a workgroup's share of the run that came into it, and of the run that leaves it.
 // kWide: a unit is a whole wave, so its keys and positions are scalars.  Keys and positions of up to `lanes` places are
 // read at once, one per lane; the rows of the next kUnroll places are in flight while those of the last are added.
-template <class T, int V, bool kWide>
-__global__ __launch_bounds__(kSumThreads) void k_embed_sum(const T* __restrict__ grad, const int* __restrict__ keys,
-                                                           const int* __restrict__ pos, int64_t n, int64_t vocab, int D,
-                                                           float scale, SumShape s, float* __restrict__ partial,
-                                                           T* __restrict__ out) {
-    __shared__ alignas(16) float heads[kSumThreads * V], tails[kSumThreads * V];
-    __shared__ int through[kSumThreads / 8];
+// heads, tails: kThreads * V floats, through: kThreads / 8 ints of LDS.
+// kAlone: there is one group, so that no run leaves it.
+template <class T, int V, bool kWide, int kThreads, bool kAlone>
+__device__ __forceinline__ void sum_places(const T* __restrict__ grad, const int* keys, const int* pos, int64_t n,
+                                           int64_t vocab, int D, float scale, const SumShape& s, int group, int slice,
+                                           float* heads, float* tails, int* through, float* __restrict__ partial,
+                                           T* __restrict__ out) {
     const int lanes = kWide ? kWave : s.lanes;
-    const int lane = threadIdx.x & (lanes - 1), unit = threadIdx.x / lanes, units = kSumThreads / lanes;
-    const int group = (int)blockIdx.x / s.slices, slice = (int)blockIdx.x - group * s.slices;
+    const int lane = threadIdx.x & (lanes - 1), unit = threadIdx.x / lanes, units = kThreads / lanes;
     const int col = (slice * lanes + lane) * V;
     const bool mine = col < D;
     const int start = !mine ? 0 : col + V <= D ? col : D - V;
@@ -428,7 +434,7 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(const T* __restrict__
     }
     __syncthreads();
     // runs that cross units: whoever they begin in adds them up
-    if (unit == 0 && came && mine) {
+    if (!kAlone && unit == 0 && came && mine) {
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = heads[threadIdx.x * V + j];
         for (int u = 0; u + 1 < units && through[u]; ++u)
@@ -448,10 +454,85 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(const T* __restrict__
             for (int j = 0; j < V; ++j) acc[j] += heads[(u * lanes + lane) * V + j];
             on = through[u];
         }
-        if (!on) write_row<T, V>(out, key, D, start, acc, scale);
+        if (kAlone || !on) write_row<T, V>(out, key, D, start, acc, scale);
         else
 #pragma unroll
             for (int j = 0; j < V; ++j) partial[((size_t)group * 2 + 1) * D + start + j] = acc[j];
+    }
+}
+
+template <class T, int V, bool kWide>
+__global__ __launch_bounds__(kSumThreads) void k_embed_sum(const T* __restrict__ grad, const int* __restrict__ keys,
+                                                           const int* __restrict__ pos, int64_t n, int64_t vocab, int D,
+                                                           float scale, SumShape s, float* __restrict__ partial,
+                                                           T* __restrict__ out) {
+    __shared__ alignas(16) float heads[kSumThreads * V], tails[kSumThreads * V];
+    __shared__ int through[kSumThreads / 8];
+    const int group = (int)blockIdx.x / s.slices, slice = (int)blockIdx.x - group * s.slices;
+    sum_places<T, V, kWide, kSumThreads, false>(grad, keys, pos, n, vocab, D, scale, s, group, slice, heads, tails, through,
+                                         partial, out);
+}
+
+// First of n sorted keys behind `at` that differs from the one before `at` (at itself for at = 0, n at most).
+__device__ __forceinline__ int run_border(const int* keys, int n, int at) {
+    if (at <= 0) return 0;
+    if (at >= n) return n;
+    const int key = keys[at - 1];
+    int lo = at, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (keys[mid] == key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Few tokens (up to kSmall): the whole gradient in one launch and without a workspace, a small step being bound by its
+// launches (1024 tokens of 8192 x 1024 in fp32, training step: 47 us, 53 in three launches).  Workgroup (group, slice)
+// sorts all tokens for itself and adds up the runs that begin in its group's places; the workgroups behind those
+// each look all tokens up for `zero_rows` rows of the table and write zeros into the rows that none names.  A run is not
+// shared among workgroups here: one token in all 1024 places takes 32 us (uniform ones 17, as in three launches), which
+// bounds kSmall.
+constexpr int kSmall = kSortThreads;
+template <class T, class I, int V, bool kWide>
+__global__ __launch_bounds__(kSortThreads) void k_embed_small(const T* __restrict__ grad, const I* __restrict__ tokens,
+                                                              int n, int64_t vocab, int64_t padding, int D, float scale,
+                                                              int passes, int bits, SumShape s, int zero_rows,
+                                                              T* __restrict__ out) {
+    __shared__ alignas(16) float heads[kSortThreads * V], tails[kSortThreads * V];
+    __shared__ int count[kSortWaves << kSortBits], through[kSortThreads / 8], part[8], sk[kSmall], sp[kSmall];
+    const int work = s.groups * s.slices;
+    if ((int)blockIdx.x < work) {
+        sort_here<1>(tokens, n, vocab, padding, passes, bits, count, part, sk, sp);
+        const int group = (int)blockIdx.x / s.slices, slice = (int)blockIdx.x - group * s.slices;
+        const int units = kSortThreads / (kWide ? kWave : s.lanes), span = units * s.len;
+        const int i0 = run_border(sk, n, group * span), i1 = run_border(sk, n, (group + 1) * span);
+        if (i0 < i1) {
+            s.len = ((i1 - i0 + units - 1) / units + kUnroll - 1) / kUnroll * kUnroll;
+            sum_places<T, V, kWide, kSortThreads, true>(grad, sk + i0, sp + i0, i1 - i0, vocab, D, scale, s, 0, slice,
+                                                        heads, tails, through, nullptr, out);
+        }
+        return;
+    }
+    int* named = sk;
+    const int64_t v0 = (int64_t)(blockIdx.x - work) * zero_rows;
+    const int rows = (int)(v0 + zero_rows < vocab ? zero_rows : vocab - v0);
+    for (int r = threadIdx.x; r < rows; r += kSortThreads) named[r] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kSortThreads) {
+        const int64_t r = (int64_t)token_key(tokens[i], vocab, padding) - v0;
+        if (r >= 0 && r < rows) named[r] = 1;
+    }
+    __syncthreads();
+    Pack<T, V> zero;
+#pragma unroll
+    for (int j = 0; j < V; ++j) zero.v[j] = from_f32<T>(0.0f);
+    const unsigned packs = (unsigned)((D + V - 1) / V);
+    for (unsigned p = threadIdx.x; p < (unsigned)rows * packs; p += kSortThreads) {
+        const unsigned r = p / packs;
+        if (named[r]) continue;
+        const int col = (int)(p - r * packs) * V;
+        store_pack<T, V>(out + (v0 + r) * D + (col + V <= D ? col : D - V), zero);
     }
 }
 

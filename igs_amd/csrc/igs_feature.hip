@@ -30,6 +30,7 @@ int embedding_shape(int64_t vocab, int D, int64_t count) {
 
 // What the dense gradient of a lookup is made of, a function of its sizes alone.
 struct EmbedPlan {
+    bool small;              // k_embed_small does all of it
     int passes, bits;        // of the sort: digits and their width
     int tiles, tile;         // more than kSortOne tokens: tiles of so many keys
     SumShape sum;
@@ -41,15 +42,19 @@ struct EmbedPlan {
 #ifndef IGS_EMBED_SUM_WAVES
 #define IGS_EMBED_SUM_WAVES 4096
 #endif
+#ifndef IGS_EMBED_SMALL
+#define IGS_EMBED_SMALL kSmall
+#endif
 #ifndef IGS_EMBED_FILL_BYTES
 #define IGS_EMBED_FILL_BYTES (64 << 10)  // per filling workgroup
 #endif
 
-EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
+EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {  // n >= 1
     EmbedPlan p;
     int total = 0;  // bits of the largest key, vocab itself
     while (vocab >> total) ++total;
     const bool one = n <= kSortOne;
+    p.small = n <= IGS_EMBED_SMALL;
     p.passes = (total + kSortBits - 1) / kSortBits;
     p.bits = (total + p.passes - 1) / p.passes;
     p.tiles = p.tile = 0;
@@ -68,13 +73,14 @@ EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {
     const int64_t waves = n * s.slices * s.lanes / kWave;
     const int64_t len = ceil_div(ceil_div(waves, IGS_EMBED_SUM_WAVES), kUnroll) * kUnroll;
     s.len = (int)(len < kUnroll ? kUnroll : len);
-    p.span = (int64_t)(kSumThreads / s.lanes) * s.len;
+    const int units = (p.small ? kSortThreads : kSumThreads) / s.lanes;
+    p.span = (int64_t)units * s.len;
     s.groups = (int)ceil_div(n, p.span);
     p.padded = ceil_div(n, 4) * 4;
     const size_t arrays = (size_t)p.padded * sizeof(int) * (one ? 2 : 4);
     p.counts_at = (arrays + 15) & ~(size_t)15;
     p.partial_at = (p.counts_at + ((size_t)p.tiles << p.bits) * sizeof(int) + 15) & ~(size_t)15;
-    p.bytes = p.partial_at + (s.groups > 1 ? (size_t)s.groups * 2 * D * sizeof(float) : 0);
+    p.bytes = p.small ? 0 : p.partial_at + (s.groups > 1 ? (size_t)s.groups * 2 * D * sizeof(float) : 0);
     return p;
 }
 
@@ -132,10 +138,23 @@ void launch_embed_sum(const T* grad, const int* keys, const int* pos, int64_t n,
                            (const float*)partial, out);
 }
 
+template <class T, class I, int V>
+void launch_embed_small(const T* grad, const I* tokens, int n, int64_t vocab, int64_t padding, int D, float scale,
+                        const EmbedPlan& p, T* out, hipStream_t st) {
+    const int64_t fit = IGS_EMBED_FILL_BYTES / ((int64_t)D * (int)sizeof(T));
+    const int rows = (int)(fit < 1 ? 1 : at_most(fit, kSmall));
+    const dim3 grid((int64_t)p.sum.groups * p.sum.slices + ceil_div(vocab, rows));
+    if (p.sum.lanes == kWave)
+        hipLaunchKernelGGL((k_embed_small<T, I, V, true>), grid, dim3(kSortThreads), 0, st, grad, tokens, n, vocab, padding,
+                           D, scale, p.passes, p.bits, p.sum, rows, out);
+    else
+        hipLaunchKernelGGL((k_embed_small<T, I, V, false>), grid, dim3(kSortThreads), 0, st, grad, tokens, n, vocab, padding,
+                           D, scale, p.passes, p.bits, p.sum, rows, out);
+}
+
 template <class T, class I>
 int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vocab, int D, float scale,
                      int64_t padding, void* out_, void* ws, hipStream_t st) {
-    const EmbedPlan p = make_embed_plan(vocab, D, sizeof(T) == 4 ? IGS_F32 : IGS_F16, n);
     T* out = (T*)out_;
     const int64_t total = vocab * D;
     // workgroups that fill `count` elements with zeros
@@ -144,6 +163,14 @@ int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vo
     };
     if (n == 0) {
         hipLaunchKernelGGL((k_fill<T>), dim3(filling(total)), dim3(kSortThreads), 0, st, out, total);
+        return launch_status();
+    }
+    const EmbedPlan p = make_embed_plan(vocab, D, sizeof(T) == 4 ? IGS_F32 : IGS_F16, n);
+    if (p.small) {
+        if (D < kVec<T>)
+            launch_embed_small<T, I, 1>((const T*)grad, (const I*)tokens, (int)n, vocab, padding, D, scale, p, out, st);
+        else
+            launch_embed_small<T, I, kVec<T>>((const T*)grad, (const I*)tokens, (int)n, vocab, padding, D, scale, p, out, st);
         return launch_status();
     }
     int *keys = (int*)ws, *pos = keys + p.padded;

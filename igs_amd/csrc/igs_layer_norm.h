@@ -5,7 +5,7 @@
 //   gx = rstd (g - mean g - h mean(g h)),  gw = sum_rows d h,  gb = sum_rows d
 //
 // Bound by memory: a row is read once and stays in registers between its sums and its result.  TPR
-// threads share a row (8 to 64 lanes of a wave, or a workgroup of 256 or 512 threads), NV packs of 16
+// threads share a row (4 to 64 lanes of a wave, 128 threads, or a workgroup of 256 or 512), NV packs of 16
 // bytes each; the weights of a thread's columns stay in registers while its workgroup walks over the
 // rows, the next row's loads in flight.  The last pack of a row whose length is no multiple of the
 // pack is moved back to end with the row: its first elements are the neighbour's (computed twice, counted
@@ -13,12 +13,13 @@
 // leaves one partial row of them, and k_norm_reduce adds those in a fixed order.
 #pragma once
 
-// Sum of up to two values over the TPR threads of a row; `red` as two buffers used in turn, so that one barrier per
-// sum is enough (a wave can be at most one sum ahead of another).
+// Sum of up to two values over the TPR threads of a row; across waves through `red`, two buffers used in turn, so that
+// one barrier per sum is enough (a wave can be at most one sum ahead of another).
+constexpr int kRedWaves = 16;  // of a workgroup, at most
 template <int TPR>
 struct RowSum {
     static constexpr int kWaves = TPR / kWave;
-    float (*red)[2][kWaves > 0 ? kWaves : 1];
+    float (*red)[2][kRedWaves];  // [turn][value][wave]
     int turn;
 
     __device__ __forceinline__ void operator()(float& a, float& b) {
@@ -28,16 +29,17 @@ struct RowSum {
         } else {
             a = lanes_sum<kWave>(a);
             b = lanes_sum<kWave>(b);
+            const int wave = threadIdx.x / kWave, first = wave & ~(kWaves - 1);
             if ((threadIdx.x & (kWave - 1)) == 0) {
-                red[turn][0][threadIdx.x / kWave] = a;
-                red[turn][1][threadIdx.x / kWave] = b;
+                red[turn][0][wave] = a;
+                red[turn][1][wave] = b;
             }
             __syncthreads();
             a = b = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                a += red[turn][0][w];
-                b += red[turn][1][w];
+                a += red[turn][0][first + w];
+                b += red[turn][1][first + w];
             }
             turn ^= 1;
         }
@@ -47,16 +49,16 @@ struct RowSum {
             a = lanes_sum<TPR>(a);
         } else {
             a = lanes_sum<kWave>(a);
-            if ((threadIdx.x & (kWave - 1)) == 0) red[turn][0][threadIdx.x / kWave] = a;
+            const int wave = threadIdx.x / kWave, first = wave & ~(kWaves - 1);
+            if ((threadIdx.x & (kWave - 1)) == 0) red[turn][0][wave] = a;
             __syncthreads();
             a = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) a += red[turn][0][w];
+            for (int w = 0; w < kWaves; ++w) a += red[turn][0][first + w];
             turn ^= 1;
         }
     }
 };
-
 constexpr int norm_threads(int tpr) { return tpr > kBlock ? tpr : kBlock; }
 
 template <class T, class W, int TPR, int NV, int V>
@@ -65,7 +67,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restr
                                                                 int64_t rows, int D, float eps, Dropout drop_,
                                                                 T* __restrict__ y, float* __restrict__ stats) {
     constexpr int kRows = norm_threads(TPR) / TPR;  // rows of a workgroup at a time
-    __shared__ float red[2][2][TPR > kWave ? TPR / kWave : 1];
+    __shared__ float red[2][2][kRedWaves];
     RowSum<TPR> row_sum{red, 0};
     const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
     const int64_t step = (int64_t)gridDim.x * kRows;
@@ -156,8 +158,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restr
                                                                 Dropout drop_, T* __restrict__ gx,
                                                                 float* __restrict__ part) {
     constexpr int kRows = norm_threads(TPR) / TPR;
-    __shared__ float red[2][2][TPR > kWave ? TPR / kWave : 1];
-    __shared__ float sums[TPR <= kWave ? 2 * TPR * NV * V : 1];
+    __shared__ float red[2][2][kRedWaves];
+    __shared__ float sums[kRows > 1 ? 2 * TPR * NV * V : 1];
     RowSum<TPR> row_sum{red, 0};
     const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
     const int64_t step = (int64_t)gridDim.x * kRows;
@@ -238,17 +240,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restr
     }
     if (!part) return;
     float* out = part + (size_t)blockIdx.x * 2 * D;
-    if constexpr (TPR > kWave) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j >= skip[k]) {
-                    out[start[k] + j] = aw[k][j];
-                    out[D + start[k] + j] = ab[k][j];
-                }
-    } else {
-        // rows of one wave by lane exchange, then the four waves one after the other
+    // the rows of a wave by lane exchange, then the workgroup's waves (TPR <= 64) or rows (128) one after the other
+    if constexpr (TPR < kWave) {
 #pragma unroll
         for (int m = TPR; m < kWave; m <<= 1)
 #pragma unroll
@@ -258,31 +251,34 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restr
                     aw[k][j] += __shfl_xor(aw[k][j], m);
                     ab[k][j] += __shfl_xor(ab[k][j], m);
                 }
-        const int wave = threadIdx.x / kWave, at = threadIdx.x & (kWave - 1);
-        for (int q = 0; q < kBlock / kWave; ++q) {
-            if (wave == q && at < TPR) {
+    }
+    constexpr int kTurn = TPR < kWave ? kWave : TPR, kTurns = kRows > 1 ? kBlock / kTurn : 1;
+    const int turn = threadIdx.x / kTurn, at = threadIdx.x % kTurn;
+    if constexpr (kTurns > 1) {
+        for (int q = kTurns - 1; q > 0; --q) {
+            if (turn == q && at < TPR) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
                         float* p = sums + ((k * V + j) * TPR + at) * 2;
-                        p[0] = q ? p[0] + aw[k][j] : aw[k][j];
-                        p[1] = q ? p[1] + ab[k][j] : ab[k][j];
+                        p[0] = q < kTurns - 1 ? p[0] + aw[k][j] : aw[k][j];
+                        p[1] = q < kTurns - 1 ? p[1] + ab[k][j] : ab[k][j];
                     }
             }
             __syncthreads();
         }
-        if (wave == 0 && at < TPR) {
+    }
+    if (turn == 0 && at < TPR) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (j >= skip[k]) {
-                        const float* p = sums + ((k * V + j) * TPR + at) * 2;
-                        out[start[k] + j] = p[0];
-                        out[D + start[k] + j] = p[1];
-                    }
-        }
+            for (int j = 0; j < V; ++j)
+                if (j >= skip[k]) {
+                    const float* p = sums + (kTurns > 1 ? ((k * V + j) * TPR + at) * 2 : 0);
+                    out[start[k] + j] = kTurns > 1 ? p[0] + aw[k][j] : aw[k][j];
+                    out[D + start[k] + j] = kTurns > 1 ? p[1] + ab[k][j] : ab[k][j];
+                }
     }
 }
 
@@ -326,7 +322,7 @@ __global__ __launch_bounds__(kLong) void k_norm_fwd_long(const T* __restrict__ x
                                                          int64_t rows, int D, float eps, Dropout drop_,
                                                          T* __restrict__ y, float* __restrict__ stats) {
     constexpr int V = kVec<T>;
-    __shared__ float red[2][2][kLong / kWave];
+    __shared__ float red[2][2][kRedWaves];
     RowSum<kLong> row_sum{red, 0};
     const PhiloxKey key = philox_key(drop_);
     const float inv = 1.0f / (float)D;
@@ -389,7 +385,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_bwd_sums(const T* __restrict__ 
                                                           const float* __restrict__ stats, int64_t rows, int D,
                                                           Dropout drop_, float2* __restrict__ sums) {
     constexpr int V = kVec<T>;
-    __shared__ float red[2][2][kBlock / kWave];
+    __shared__ float red[2][2][kRedWaves];
     RowSum<kBlock> row_sum{red, 0};
     const PhiloxKey key = philox_key(drop_);
     const float inv = 1.0f / (float)D;

@@ -23,8 +23,8 @@ int norm_shape(int64_t rows, int D, int dtype, int wdtype) {
 }
 
 // How a row of D elements is laid over threads: TPR threads of NV packs of V elements, the smallest
-// arrangement that holds the row.  A wave of up to 16 elements per thread, a workgroup of 256 threads of up
-// to 32, one of 512 (24 or 32).  The backward, which has x, gy, h, d, w and the two sums of every element in
+// arrangement that holds the row.  A wave or 128 threads of up to 16 elements each, a workgroup of 256 threads of
+// up to 32, one of 512 (24 or 32).  The backward, which has x, gy, h, d, w and the two sums of every element in
 // registers, takes no more than 16 (kTwoPass elements a row); wider rows go in two kernels there.
 struct NormShape {
     int tpr, nv;
@@ -40,7 +40,8 @@ NormShape norm_layout(int D, int dtype) {
         if (packs <= tpr) return {tpr, 1, false, false};
     for (int nv = 2; nv <= 2 * unit; nv *= 2)
         if (packs <= kWave * nv) return {kWave, nv, false, false};
-    for (int k = 1; k <= 4; ++k)
+    if (packs <= 128 * 2 * unit) return {128, 2 * unit, false, false};
+    for (int k = 2; k <= 4; ++k)
         if (packs <= 256 * k * unit) return {256, k * unit, false, false};
     for (int k = 3; k <= 4; ++k)
         if (packs <= 512 * k * unit) return {512, k * unit, false, false};
@@ -71,7 +72,7 @@ inline int norm_elements(const NormShape& s, int dtype) { return s.one ? 1 : s.n
 // Workgroups per compute unit: each loads the weights of its columns once and, in the backward, leaves a
 // partial row of 2 D sums, so few workgroups that walk over many rows, but enough to keep the memory busy
 // (us at 2 / 4 / 6 per compute unit, backward: bf16 32768 x 1024 40 / 45 / 50, fp32 4096 x 4096
-// 46 / 57 / 69, bf16 16384 x 2048 64 / 52 / 65, bf16 65536 x 256 25 / 23 / 27).
+// 46 / 57 / 69, bf16 65536 x 256 25 / 23 / 27).
 int64_t norm_fwd_groups(const NormShape& s, int64_t rows, int dtype) {
     const int per_cu = s.tpr > kBlock ? IGS_NORM_FWD_WGS_512 : norm_elements(s, dtype) > 16 ? IGS_NORM_FWD_WGS_WIDE : IGS_NORM_FWD_WGS;
     return at_most(ceil_div(rows, norm_rows_at_once(s)), (int64_t)device_cus() * per_cu);
@@ -120,7 +121,7 @@ void norm_dispatch(const NormShape& s, F f) {  // rows of up to kTwoPass element
         if (s.nv == 2) return f(NormLayout<64, 2, V>());
         return f(NormLayout<64, 2 * U, V>());
     }
-    if (s.nv == U) return f(NormLayout<256, U, V>());
+    if (s.tpr == 128) return f(NormLayout<128, 2 * U, V>());
     return f(NormLayout<256, 2 * U, V>());
 }
 template <class T, class F>
