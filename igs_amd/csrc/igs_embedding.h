@@ -16,29 +16,30 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
                                                       int D, const I* __restrict__ tokens, int64_t count,
                                                       float scale, int lanes, T* __restrict__ out) {
     const int per = kBlock / lanes, slot = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
-    const int64_t i = (int64_t)blockIdx.x * (per * U) + slot;
-    const T* src[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t at = i + u * per;
-        const I t = at < count ? tokens[at] : (I)0;
-        ok[u] = token_ok(t, vocab);
-        src[u] = weight + (ok[u] ? (int64_t)t : 0) * stride;
-    }
-    for (int d = lane * V; d < D; d += lanes * V) {
-        const int col = d + V <= D ? d : D - V;
-        Pack<T, V> q[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = load_pack<T, V>(src[u] + col);
+    for (int64_t i = (int64_t)blockIdx.x * (per * U) + slot; i < count; i += (int64_t)gridDim.x * (per * U)) {
+        const T* src[U];
+        bool ok[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = i + u * per;
-            if (at >= count) break;
+            const I t = at < count ? tokens[at] : (I)0;
+            ok[u] = token_ok(t, vocab);
+            src[u] = weight + (ok[u] ? (int64_t)t : 0) * stride;
+        }
+        for (int d = lane * V; d < D; d += lanes * V) {
+            const int col = d + V <= D ? d : D - V;
+            Pack<T, V> q[U];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                q[u].v[j] = ok[u] ? from_f32<T>(to_f32(q[u].v[j]) * scale) : from_f32<T>(__builtin_nanf(""));
-            store_pack<T, V>(out + at * D + col, q[u]);
+            for (int u = 0; u < U; ++u) q[u] = load_pack<T, V>(src[u] + col);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = i + u * per;
+                if (at >= count) break;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    q[u].v[j] = ok[u] ? from_f32<T>(to_f32(q[u].v[j]) * scale) : from_f32<T>(__builtin_nanf(""));
+                store_pack<T, V>(out + at * D + col, q[u]);
+            }
         }
     }
 }

@@ -107,7 +107,7 @@ int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, c
     const int per = kBlock / lanes;
     // four tokens in flight per thread where that still leaves eight workgroups per compute unit
     const bool four = ceil_div(count, 4 * per) >= 8 * (int64_t)device_cus();
-    const dim3 grid(ceil_div(count, four ? 4 * per : per));
+    const dim3 grid(at_most(ceil_div(count, four ? 4 * per : per), 1 << 23));
 #define IGS_EMBED_FWD(VV, U)                                                                                    \
     hipLaunchKernelGGL((k_embed_fwd<T, I, VV, U>), grid, dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D, \
                        (const I*)tokens, count, scale, lanes, (T*)out)
@@ -142,7 +142,8 @@ template <class T, class I, int V>
 void launch_embed_small(const T* grad, const I* tokens, int n, int64_t vocab, int64_t padding, int D, float scale,
                         const EmbedPlan& p, T* out, hipStream_t st) {
     const int64_t fit = IGS_EMBED_FILL_BYTES / ((int64_t)D * (int)sizeof(T));
-    const int rows = (int)(fit < 1 ? 1 : at_most(fit, kSmall));
+    const int64_t least = ceil_div(vocab, 1 << 21);  // a launch has fewer than 2^32 threads
+    const int rows = (int)(fit < least ? least : at_most(fit, kSmall));
     const dim3 grid((int64_t)p.sum.groups * p.sum.slices + ceil_div(vocab, rows));
     if (p.sum.lanes == kWave)
         hipLaunchKernelGGL((k_embed_small<T, I, V, true>), grid, dim3(kSortThreads), 0, st, grad, tokens, n, vocab, padding,

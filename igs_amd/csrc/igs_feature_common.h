@@ -82,6 +82,11 @@ __device__ __forceinline__ PhiloxKey philox_key(const Dropout& d) {
     return k;
 }
 
+// a ^ b ^ c in one instruction
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+    return (uint32_t)__builtin_amdgcn_bitop3_b32((int)a, (int)b, (int)c, 0x96);
+}
+
 // Philox4x32, seven rounds (Salmon, Moraes, Dror, Shaw 2011: the fewest that pass their test batteries;
 // dropout asks no more of its numbers).  128 bits per block serve eight elements with 16 bits each,
 // which keeps the integer products (quarter rate) below the time of the memory traffic.
@@ -91,9 +96,9 @@ __device__ __forceinline__ void philox(uint64_t block, const PhiloxKey& key, uin
 #pragma unroll
     for (int r = 0; r < 7; ++r) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = xor3((uint32_t)(b >> 32), c1, k0);
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = xor3((uint32_t)(a >> 32), c3, k1);
         c3 = (uint32_t)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;

@@ -99,9 +99,34 @@ std::tuple<Tensor, int64_t> rows_of(const Tensor& x) {
     return {x, step < 0 ? D : step};
 }
 
+// The registered operators can be called directly, so what would make a kernel read beside a tensor is checked here.
+void same_device(const Tensor& a, const Tensor& b, const char* what) {
+    TORCH_CHECK(!b.defined() || b.device() == a.device(), "Expected all tensors to be on the same device, but ", what, " is on ",
+                b.defined() ? b.device() : a.device(), " and the first tensor on ", a.device());
+}
+void check_tokens(const Tensor& tokens) {
+    TORCH_CHECK(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int32 or int64");
+}
+void check_weights(const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    for (const Tensor* t : {&weight, &bias})
+        if (t->defined()) {
+            same_device(x, *t, "a weight");
+            TORCH_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), "weight and bias must be [", x.size(-1), "]");
+        }
+    TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
+                "weight and bias must have one type");
+}
+void check_grad(const Tensor& grad, const Tensor& like, int64_t numel) {
+    same_device(like, grad, "the upstream gradient");
+    TORCH_CHECK(grad.scalar_type() == like.scalar_type() && grad.numel() == numel, "the upstream gradient has another type or size");
+}
+
 // ---------------------------------------------------------------------------------- library calls
 Tensor embedding_fwd(const Tensor& tokens_, const Tensor& weight_, double scale) {
     const c10::OptionalDeviceGuard guard(weight_.device());
+    check_tokens(tokens_);
+    same_device(weight_, tokens_, "tokens");
+    TORCH_CHECK(weight_.dim() == 2, "weight must be [V, D]");
     const Tensor tokens = tokens_.contiguous();
     const int64_t vocab = weight_.size(0), D = weight_.size(1);
     const Tensor weight = D > 1 && weight_.stride(1) != 1 ? weight_.contiguous() : weight_;
@@ -117,6 +142,9 @@ Tensor embedding_fwd(const Tensor& tokens_, const Tensor& weight_, double scale)
 
 Tensor embedding_bwd(const Tensor& grad_, const Tensor& tokens_, int64_t vocab, double scale, int64_t padding) {
     const c10::OptionalDeviceGuard guard(grad_.device());
+    check_tokens(tokens_);
+    same_device(grad_, tokens_, "tokens");
+    TORCH_CHECK(grad_.dim() > 0 && grad_.numel() == tokens_.numel() * grad_.size(-1), "one gradient row per token");
     const Tensor grad = grad_.contiguous(), tokens = tokens_.contiguous();
     const int64_t D = grad.size(-1), n = tokens.numel();
     const int code = dtype_code(grad);
@@ -134,11 +162,19 @@ struct DropoutArgs {
     int64_t threshold, seed;
     Tensor seed_tensor;
     int64_t offset;
+    void check(const Tensor& x) const {
+        same_device(x, seed_tensor, "the seed");
+        TORCH_CHECK(!seed_tensor.defined() || (seed_tensor.scalar_type() == at::kLong && seed_tensor.numel() == 1),
+                    "a seed tensor holds one int64 element");
+    }
 };
 
 std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, double eps,
                                     const DropoutArgs& d, bool want_stats) {
     const c10::OptionalDeviceGuard guard(x_.device());
+    TORCH_CHECK(x_.dim() > 0 && x_.size(-1) > 0, "x must have a last axis of one element or more");
+    check_weights(x_, weight_, bias_);
+    d.check(x_);
     const auto [x, step] = rows_of(x_);
     const Tensor weight = weight_.defined() ? weight_.contiguous() : weight_, bias = bias_.defined() ? bias_.contiguous() : bias_;
     const int64_t D = x.size(-1), rows = x.numel() / D;
@@ -157,9 +193,16 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
                                             at::ScalarType wtype, const Tensor& stats, const DropoutArgs& d, bool want_x,
                                             bool want_w, bool want_b) {
     const c10::OptionalDeviceGuard guard(x_.device());
+    TORCH_CHECK(x_.dim() > 0 && x_.size(-1) > 0, "x must have a last axis of one element or more");
+    check_weights(x_, weight_, Tensor());
+    check_grad(grad_, x_, x_.numel());
+    d.check(x_);
+    same_device(x_, stats, "the statistics");
+    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * (x_.numel() / x_.size(-1)),
+                "the statistics are the forward's");
     const auto [x, step] = rows_of(x_);
     const Tensor grad = grad_.contiguous(), weight = weight_.defined() ? weight_.contiguous() : weight_;
-    const int64_t D = x.size(-1), rows = stats.size(0);
+    const int64_t D = x.size(-1), rows = x.numel() / D;
     const auto wopts = x.options().dtype(wtype);
     const Tensor gx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor gw = want_w ? at::empty({D}, wopts) : Tensor(), gb = want_b ? at::empty({D}, wopts) : Tensor();
@@ -179,6 +222,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
 
 Tensor dropout_call(const Tensor& x_, const DropoutArgs& d) {
     const c10::OptionalDeviceGuard guard(x_.device());
+    d.check(x_);
     const Tensor x = x_.contiguous(), y = at::empty(x.sizes(), x.options());
     check(lib.dropout(address(x), dtype_code(x), x.numel(), static_cast<int>(d.threshold), static_cast<uint64_t>(d.seed),
                       seed_address(d.seed_tensor), static_cast<uint64_t>(d.offset), writable(y), stream_of(x)),

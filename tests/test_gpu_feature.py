@@ -251,7 +251,7 @@ def test_layer_norm(igs, dev, dtype, wdtype, R, D, p):
         assert torch.equal(one, grads[k])
 
 
-@pytest.mark.parametrize("R,D", [(5000, 24), (3001, 130), (2053, 1024), (20000, 8), (1100, 2050)])
+@pytest.mark.parametrize("R,D", [(5000, 24), (3001, 130), (2053, 1024), (20000, 8), (701, 1500), (1100, 2050), (1030, 5000), (150, 20003)])
 def test_layer_norm_weight_gradient_over_many_rows(igs, dev, R, D):
     for dtype in DTYPES:
         x, up = normal((R, D), R, dtype, 0.4, 1.7), normal((R, D), D, dtype)
@@ -508,16 +508,20 @@ def test_training_step_is_graph_capturable(igs, dev):
             step()
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = step()
+    with torch.cuda.graph(other):                        # a second one: neither may work in the other's buffers
+        out2 = step()
     for k in (5, 6, 5, 2 ** 60):
         seed.fill_(k)
         up.add_(0.25)
         graph.replay()
+        other.replay()
         torch.cuda.synchronize()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(out2, want))
     assert not torch.equal(igs.dropout(w, 0.5, 1), igs.dropout(w, 0.5, 2))
     assert not torch.equal(igs.dropout(w, 0.5, 1, 0), igs.dropout(w, 0.5, 1, 1))
 
@@ -565,6 +569,23 @@ def test_mixed_devices_raise(igs, dev):
         igs.layer_norm(x, torch.ones(4))
     with pytest.raises(RuntimeError, match="same device"):
         igs.dropout(x, 0.5, torch.tensor([1]))
+    ops = torch.ops.igs_amd                             # the registered operators, called directly
+    for call in (lambda: ops.embedding_fwd(t, w, 1.0, -1), lambda: ops.embedding_fwd(x[0], w, 1.0, -1),
+                 lambda: ops.embedding_fwd(t.to(dev), w[0], 1.0, -1), lambda: ops.embedding_bwd(x, t.to(dev), 5, 1.0, -1),
+                 lambda: ops.embedding_bwd(x[:1], t, 5, 1.0, -1), lambda: ops.layer_norm_fwd(x, w[0, :3], None, 1e-5, 0, 0, None, 0),
+                 lambda: ops.layer_norm_fwd(x, w[0], w[0].half(), 1e-5, 0, 0, None, 0),
+                 lambda: ops.layer_norm_fwd(x, torch.ones(4), None, 1e-5, 0, 0, None, 0),
+                 lambda: ops.layer_norm_bwd(x[:2], x, None, None, torch.zeros(3, 2, device=dev), 0, 0, None, 0),
+                 lambda: ops.layer_norm_bwd(x.half(), x, None, None, torch.zeros(3, 2, device=dev), 0, 0, None, 0),
+                 lambda: ops.layer_norm_bwd(x, x, None, None, torch.zeros(2, 2, device=dev), 0, 0, None, 0),
+                 lambda: ops.dropout(x, 9, 0, torch.zeros(2, device=dev, dtype=torch.int64), 0),
+                 lambda: ops.dropout(x.double(), 9, 0, None, 0), lambda: ops.dropout(x, 70000, 0, None, 0)):
+        with pytest.raises(RuntimeError):
+            call()
+    # an upstream gradient of another type is converted, as torch does
+    leaf = x.half().requires_grad_(True)
+    (g,) = torch.autograd.grad(igs.dropout(leaf, 0.5, 1), leaf, torch.ones(3, 4, device=dev))
+    assert g.dtype == torch.float16 and torch.equal(g, igs.dropout(torch.ones(3, 4, device=dev).half(), 0.5, 1))
 
 
 # ---------------------------------------------------------------------------------- the module
@@ -626,3 +647,12 @@ def test_compiled_operators(igs, dev):
         res.append((y.detach(), *torch.autograd.grad(y, lv, up)))
     for a, b in zip(*res):
         assert torch.equal(a, b)
+    m = igs.GaussianSplatting2D(4, 72, num_embeddings=70, feature_norm=True, feature_dropout=0.2).to(dev)
+    m.dropout_seed = seed
+    ids = t[:24].view(2, 12)
+    torch._dynamo.reset()
+    want, got = m(ids, size=(9, 11)), torch.compile(lambda v: m(v, size=(9, 11)), fullgraph=True)(ids)
+    assert torch.allclose(got[1], want[1], rtol=1e-5, atol=1e-6) and torch.allclose(got[0], want[0], rtol=1e-4, atol=1e-5)
+    m.dropout_seed = None                                # a seed drawn on the device inside the graph
+    torch.compile(lambda v: m(v, size=(9, 11)), fullgraph=True)(ids)[0].sum().backward()
+    assert bool(m.embedding.weight.grad.isfinite().all()) and bool(m.embedding.weight.grad.any())
