@@ -11,7 +11,7 @@ __device__ __forceinline__ bool token_ok(I t, int64_t vocab) {
 // token and walk its row in packs of V elements; the last pack of a row of another length is moved back
 // to end with the row.  Rows of fewer elements than a pack go with V = 1.  A thread has the packs of U
 // tokens in flight: a single gather per thread leaves the memory idle between id, row and store.
-template <class T, class I, int V, int U>
+template <class T, class I, int V, int U, bool kStream>
 __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weight, int64_t stride, int64_t vocab,
                                                       int D, const I* __restrict__ tokens, int64_t count,
                                                       float scale, int lanes, T* __restrict__ out) {
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     q[u].v[j] = ok[u] ? from_f32<T>(to_f32(q[u].v[j]) * scale) : from_f32<T>(__builtin_nanf(""));
-                store_pack<T, V>(out + at * D + col, q[u]);
+                store_pack<kStream, T, V>(out + at * D + col, q[u]);
             }
         }
     }
@@ -84,15 +84,20 @@ __device__ __forceinline__ int token_key(I t, int64_t vocab, int64_t padding) {
     return token_ok(t, vocab) && (int64_t)t != padding ? (int)t : (int)vocab;
 }
 
-// Lanes of the wave whose digit is this lane's (`active`: the lanes that hold a key).
+// Lanes of the wave with this lane's digit, among those that hold a key (`valid`).  Per bit: the lanes where it is set, as
+// a scalar, and two three-input operations, m & ~(set ^ mine).
 __device__ __forceinline__ uint64_t match_digit(int digit, int bits, bool valid) {
-    uint64_t m = __ballot(valid);
-    for (int b = 0; b < bits; ++b) {
-        const bool set = (digit >> b) & 1;
-        const uint64_t v = __ballot(set);
-        m &= set ? v : ~v;
+    const uint64_t all = __ballot(valid);
+    int lo = (int)(uint32_t)all, hi = (int)(uint32_t)(all >> 32);
+#pragma unroll
+    for (int b = 0; b < kSortBits; ++b) {
+        if (b >= bits) break;  // uniform
+        const int mine = (int)((uint32_t)digit << (31 - b)) >> 31;
+        const uint64_t set = __ballot(mine != 0);
+        lo = __builtin_amdgcn_bitop3_b32(lo, (int)(uint32_t)set, mine, 0x90);
+        hi = __builtin_amdgcn_bitop3_b32(hi, (int)(uint32_t)(set >> 32), mine, 0x90);
     }
-    return m;
+    return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
 }
 __device__ __forceinline__ int lanes_below(uint64_t m) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
@@ -333,7 +338,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortSource<I> src, 
 // `lanes` packs of the row; a workgroup's units are neighbours (span = units * len places).
 struct SumShape {
     int lanes, slices, len;
-    int groups;  // workgroups per slice
+    int groups;   // workgroups per slice
+    bool stream;  // the upstream gradient is read past the caches
 };
 
 template <class T, int V>
@@ -386,7 +392,7 @@ __device__ __forceinline__ void sum_places(const T* __restrict__ grad, const int
                 for (int u = 0; u < kUnroll; ++u) {
                     if (q + u >= places) break;
                     const int k = of(kv, q + u), i = of(pv, q + u);  // all lanes of the unit: one of them holds the values
-                    if (k != none && mine) g[u] = load_pack<T, V>(grad + (int64_t)i * D + start);
+                    if (k != none && mine) g[u] = load_pack<T, V>(grad + (int64_t)i * D + start, s.stream);
                 }
             };
             const auto add = [&](const Pack<T, V> (&g)[kUnroll], int q) {

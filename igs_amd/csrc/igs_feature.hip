@@ -76,6 +76,7 @@ EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {  // n >=
     const int units = (p.small ? kSortThreads : kSumThreads) / s.lanes;
     p.span = (int64_t)units * s.len;
     s.groups = (int)ceil_div(n, p.span);
+    s.stream = n * D * dtype_bytes(dtype) >= kStreamBytes;
     p.padded = ceil_div(n, 4) * 4;
     const size_t arrays = (size_t)p.padded * sizeof(int) * (one ? 2 : 4);
     p.counts_at = (arrays + 15) & ~(size_t)15;
@@ -106,17 +107,19 @@ int launch_embed_fwd(const void* weight, int64_t stride, int64_t vocab, int D, c
     while (lanes < packs && lanes < kBlock) lanes *= 2;
     const int per = kBlock / lanes;
     // four tokens in flight per thread where that still leaves eight workgroups per compute unit
-    const bool four = ceil_div(count, 4 * per) >= 8 * (int64_t)device_cus();
+    const bool stream = count * D * (int64_t)sizeof(T) >= kStreamBytes;
+    const bool four = (stream && D >= V) || ceil_div(count, 4 * per) >= 8 * (int64_t)device_cus();
     const dim3 grid(at_most(ceil_div(count, four ? 4 * per : per), 1 << 23));
-#define IGS_EMBED_FWD(VV, U)                                                                                    \
-    hipLaunchKernelGGL((k_embed_fwd<T, I, VV, U>), grid, dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D, \
+#define IGS_EMBED_FWD(VV, U, S)                                                                                   \
+    hipLaunchKernelGGL((k_embed_fwd<T, I, VV, U, S>), grid, dim3(kBlock), 0, st, (const T*)weight, stride, vocab, D, \
                        (const I*)tokens, count, scale, lanes, (T*)out)
     if (D < V) {
-        if (four) IGS_EMBED_FWD(1, 4);
-        else IGS_EMBED_FWD(1, 1);
+        if (four) IGS_EMBED_FWD(1, 4, false);
+        else IGS_EMBED_FWD(1, 1, false);
     } else {
-        if (four) IGS_EMBED_FWD(V, 4);
-        else IGS_EMBED_FWD(V, 1);
+        if (stream) IGS_EMBED_FWD(V, 4, true);
+        else if (four) IGS_EMBED_FWD(V, 4, false);
+        else IGS_EMBED_FWD(V, 1, false);
     }
 #undef IGS_EMBED_FWD
     return launch_status();

@@ -36,6 +36,33 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& q) {
     *reinterpret_cast<Pack<T, V>*>(p) = q;
 }
 
+// The same past the caches (non-temporal), for tensors that the last-level cache cannot hold anyway: what it does hold
+// then stays.  `stream` is uniform; a call streams what it reads (lookup: writes) in kStreamBytes or more.  us without / with:
+// norm bf16 x 1024, rows 65536 forward 44 / 45, backward 77 / 69; 131072 98 / 84, 148 / 129; 32768 23 / 24, 39 / 39;
+// lookup of 131072 tokens of 65536 x 1024 in bf16 83 / 57 (stores), its gradient 131 / 121.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p, bool stream) {
+    if constexpr (sizeof(Pack<T, V>) == 16) {
+        if (stream) {
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+            return __builtin_bit_cast(Pack<T, V>, v);
+        }
+    }
+    return load_pack<T, V>(p);
+}
+// (a constant here: the compiler makes one store of the two of a branch, an ordinary one)
+template <bool kStream, class T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& q) {
+    if constexpr (kStream && sizeof(Pack<T, V>) == 16) {
+        const u32x4_any v = __builtin_bit_cast(u32x4, q);
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));
+    } else {
+        store_pack<T, V>(p, q);
+    }
+}
+
 // Sums over the TPR lanes of a row within a wave (TPR = 4, 8, 16, 32 or 64), the same bits in all of them.
 // Every lane of the wave takes part.  Data-parallel moves inside 16 lanes; a whole wave's four sums
 // of 16 are read as scalars.

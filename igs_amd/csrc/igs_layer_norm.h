@@ -64,7 +64,7 @@ constexpr int norm_threads(int tpr) { return tpr > kBlock ? tpr : kBlock; }
 template <class T, class W, int TPR, int NV, int V>
 __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restrict__ x, int64_t stride,
                                                                 const W* __restrict__ w, const W* __restrict__ b,
-                                                                int64_t rows, int D, float eps, Dropout drop_,
+                                                                int64_t rows, int D, float eps, Dropout drop_, bool stream,
                                                                 T* __restrict__ y, float* __restrict__ stats) {
     constexpr int kRows = norm_threads(TPR) / TPR;  // rows of a workgroup at a time
     __shared__ float red[2][2][kRedWaves];
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restr
         const T* p = x + r * stride;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-            if (skip[k] < V) next[k] = load_pack<T, V>(p + start[k]);
+            if (skip[k] < V) next[k] = load_pack<T, V>(p + start[k], stream);
     };
     if (r0 < rows) load(r0);
     for (; r0 < rows; r0 += step) {
@@ -155,7 +155,7 @@ template <class T, class W, int TPR, int NV, int V>
 __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restrict__ gy, const T* __restrict__ x,
                                                                 int64_t stride, const W* __restrict__ w,
                                                                 const float* __restrict__ stats, int64_t rows, int D,
-                                                                Dropout drop_, T* __restrict__ gx,
+                                                                Dropout drop_, bool stream, T* __restrict__ gx,
                                                                 float* __restrict__ part) {
     constexpr int kRows = norm_threads(TPR) / TPR;
     __shared__ float red[2][2][kRedWaves];
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_bwd(const T* __restr
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (skip[k] < V) {
-                nx[k] = load_pack<T, V>(x + r * stride + start[k]);
-                ng[k] = load_pack<T, V>(gy + r * D + start[k]);
+                nx[k] = load_pack<T, V>(x + r * stride + start[k], stream);
+                ng[k] = load_pack<T, V>(gy + r * D + start[k], stream);
             }
         ns = reinterpret_cast<const float2*>(stats)[r];
     };

@@ -144,7 +144,7 @@ int launch_norm_fwd(const void* x, int64_t stride, const void* w, const void* b,
         using L = decltype(l);
         hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v>), dim3(norm_fwd_groups(s, rows, dtype)),
                            dim3(norm_threads(L::tpr)), 0, st, (const T*)x, stride, (const W*)w, (const W*)b, rows, D, eps,
-                           d, (T*)y, stats);
+                           d, rows * D * (int64_t)sizeof(T) >= kStreamBytes, (T*)y, stats);
     };
     if (s.is_long)
         hipLaunchKernelGGL((k_norm_fwd_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)x, stride,
@@ -175,7 +175,8 @@ int launch_norm_bwd(const void* gy, const void* x, int64_t stride, const void* w
         norm_dispatch<T>(norm_layout(D, dtype), [&](auto l) {
             using L = decltype(l);
             hipLaunchKernelGGL((k_norm_bwd<T, W, L::tpr, L::nv, L::v>), dim3(partials), dim3(norm_threads(L::tpr)), 0, st,
-                               (const T*)gy, (const T*)x, stride, (const W*)w, stats, rows, D, d, (T*)gx, part);
+                               (const T*)gy, (const T*)x, stride, (const W*)w, stats, rows, D, d,
+                               2 * rows * D * (int64_t)sizeof(T) >= kStreamBytes, (T*)gx, part);
         });
     }
     if (sums)

@@ -430,6 +430,35 @@ def test_offsets_beyond_32_bits(igs, dev):
     assert bool((g[-1] == 2).all()) and bool((g[V // 2] == 1).all()) and float(g[:: 4096].float().sum()) == (D if (V // 2) % 4096 == 0 else 0) + (2 * D if (V - 1) % 4096 == 0 else 0)
 
 
+def test_tensors_larger_than_the_caches(igs, dev):
+    """Tensors that are read and written past the caches give what the cached ones give: the lookup's gradient of whole
+    numbers is exact, and a norm's rows do not depend on how many there are."""
+    n, V, D = 100003, 700, 1024
+    g = torch.Generator(dev).manual_seed(1)
+    t = torch.randint(0, V, (n,), generator=g, device=dev)
+    up = torch.randint(-1, 2, (n, D), generator=g, device=dev, dtype=torch.int8).to(torch.bfloat16)
+    w = torch.randn(V, D, generator=g, device=dev).to(torch.bfloat16).requires_grad_(True)
+    y = igs.embedding_lookup(t, w)
+    assert torch.equal(y, w.detach()[t])
+    (got,) = torch.autograd.grad(y, w, up)
+    want = torch.zeros(V, D, device=dev).index_add_(0, t, up.float())     # whole numbers below 2^24: exact in any order
+    assert torch.equal(got, want.to(torch.bfloat16))
+    x = y.detach().requires_grad_(True)
+    z = igs.layer_norm(x, dropout_p=0.25, seed=3)
+    (gx,) = torch.autograd.grad(z, x, up)
+    for r in (0, 50000, n - 9):
+        part = x.detach()[r:r + 9].clone().requires_grad_(True)
+        f = igs.layer_norm(part)
+        keep = igs.dropout_keep_mask((n * D,), 0.25, 3, device=dev).view(n, D)[r:r + 9]
+        # (the masked gradient of the slice is rounded to bf16, 2^-9 of each of the three terms of its rows)
+        masked = torch.where(keep, up[r:r + 9].float() * (65536 / (65536 - 16384)), 0.0)
+        (gp,) = torch.autograd.grad(f, part, masked.to(torch.bfloat16))
+        assert torch.equal(z[r:r + 9] == 0, ~keep | (z[r:r + 9] == 0))
+        assert torch.allclose(gx[r:r + 9].float(), gp.float(), rtol=2 ** -7, atol=1e-2 * float(gp.float().abs().max()))
+        whole = igs.layer_norm(x.detach())[r:r + 9]
+        assert torch.equal(whole, f.detach())
+
+
 # ---------------------------------------------------------------------------------- together, streams, graphs
 def chain(igs, t, w, gw, gb, seed):
     f = igs.embedding_lookup(t, w, 1.5, 0)
