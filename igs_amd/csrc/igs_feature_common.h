@@ -37,9 +37,10 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& q) {
 }
 
 // The same past the caches (non-temporal), for tensors that the last-level cache cannot hold anyway: what it does hold
-// then stays.  `stream` is uniform; a call streams what it reads (lookup: writes) in kStreamBytes or more.  us without / with:
-// norm bf16 x 1024, rows 65536 forward 44 / 45, backward 77 / 69; 131072 98 / 84, 148 / 129; 32768 23 / 24, 39 / 39;
-// lookup of 131072 tokens of 65536 x 1024 in bf16 83 / 57 (stores), its gradient 131 / 121.
+// then stays.  `stream` is uniform; a call does so from kStreamBytes of reads (lookup and norm with a backward: writes)
+// on.  us without / with, each call by itself: norm bf16 x 1024, 32768 rows forward 23 / 24, backward 39 / 39; 65536 rows
+// 44 / 45, 77 / 69; 131072 rows 98 / 84, 148 / 129; lookup of 131072 tokens of 65536 x 1024 in bf16 83 / 57 (stores),
+// its gradient 131 / 112.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <class T, int V>

@@ -8,8 +8,7 @@ constexpr int kMaxRow = 1 << 20;
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t at_most(int64_t v, int64_t most) { return v < most ? v : most; }
 
-// From so many bytes on a tensor is read (the lookup's result: written) past the caches: three quarters of the
-// last-level cache.
+// From so many bytes on a tensor is read or written past the caches: three quarters of the last-level cache.
 constexpr int64_t kStreamBytes = 192ll << 20;
 
 inline int launch_status() {

@@ -61,7 +61,7 @@ struct RowSum {
 };
 constexpr int norm_threads(int tpr) { return tpr > kBlock ? tpr : kBlock; }
 
-template <class T, class W, int TPR, int NV, int V>
+template <class T, class W, int TPR, int NV, int V, bool kStreamOut>
 __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restrict__ x, int64_t stride,
                                                                 const W* __restrict__ w, const W* __restrict__ b,
                                                                 int64_t rows, int D, float eps, Dropout drop_, bool stream,
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void k_norm_fwd(const T* __restr
                     if (drop_.threshold) drop<V>(c[k], (uint64_t)r * D + start[k], whole, drop_, key);
 #pragma unroll
                     for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(c[k][j]);
-                    store_pack<T, V>(y + r * D + start[k], q);
+                    store_pack<kStreamOut, T, V>(y + r * D + start[k], q);
                 }
             if (stats && lane == 0) {
                 stats[2 * r] = mean;

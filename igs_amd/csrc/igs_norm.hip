@@ -140,11 +140,18 @@ int launch_norm_fwd(const void* x, int64_t stride, const void* w, const void* b,
                     const Dropout& d, void* y, float* stats, hipStream_t st) {
     constexpr int dtype = sizeof(T) == 4 ? IGS_F32 : IGS_F16;
     const NormShape s = norm_layout(D, dtype);
+    // Past the caches goes y where a backward follows (bf16 131072 x 1024, forward and backward 250 us without, 240
+    // with it; 249 with x instead), and x where none does (forward 98 us without, 84 with x, 95 with y).
+    const bool large = rows * D * (int64_t)sizeof(T) >= kStreamBytes;
     const auto launch = [&](auto l) {
         using L = decltype(l);
-        hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v>), dim3(norm_fwd_groups(s, rows, dtype)),
-                           dim3(norm_threads(L::tpr)), 0, st, (const T*)x, stride, (const W*)w, (const W*)b, rows, D, eps,
-                           d, rows * D * (int64_t)sizeof(T) >= kStreamBytes, (T*)y, stats);
+        const dim3 grid(norm_fwd_groups(s, rows, dtype)), threads(norm_threads(L::tpr));
+        if (large && stats)
+            hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v, true>), grid, threads, 0, st, (const T*)x, stride,
+                               (const W*)w, (const W*)b, rows, D, eps, d, false, (T*)y, stats);
+        else
+            hipLaunchKernelGGL((k_norm_fwd<T, W, L::tpr, L::nv, L::v, false>), grid, threads, 0, st, (const T*)x, stride,
+                               (const W*)w, (const W*)b, rows, D, eps, d, large, (T*)y, stats);
     };
     if (s.is_long)
         hipLaunchKernelGGL((k_norm_fwd_long<T, W>), dim3(at_most(rows, 1 << 20)), dim3(kLong), 0, st, (const T*)x, stride,
