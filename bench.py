@@ -100,6 +100,11 @@ def main() -> int:
                          "diversity loss (src/igs/reg.py of the reference) beside the plain torch expression")
     ap.add_argument("--koleo-shape", default=None, metavar="BxNxD",
                     help="with --koleo: time this one shape only, without the torch and CPU columns (for profiling)")
+    ap.add_argument("--features", action="store_true",
+                    help="instead of the JSON line, time the feature operators (embedding lookup, layer norm, dropout) over the "
+                         "cases of perf/operators.py, beside their plain torch forms")
+    ap.add_argument("--feature-case", default=None, metavar="NAME",
+                    help="with --features: this one case only, without the plain form (for profiling)")
     ap.add_argument("--skip-tolerance", type=float, default=None, metavar="T",
                     help="bound on what skipped pairs may change in an output element, as a fraction of the largest "
                          "colour (default: the library's 1e-7; 0 = skip exact zeros only)")
@@ -135,6 +140,8 @@ def run(args) -> int:
         return all_configs(args.steps, args.warmup, args.no_cpu)
     if args.koleo:
         return koleo_table(args.no_cpu, args.koleo_shape)
+    if args.features:
+        return feature_table(args.feature_case)
     if args.fit:
         return fit_step(args.config, args.steps, args.warmup)
 
@@ -723,6 +730,43 @@ def koleo_table(no_cpu: bool, only: str = None) -> int:
             cpu = (time.perf_counter() - t0) * 1e3
         print("%-16s %10.4f %10.4f %12.4f %12.4f %12.2f %10.1f" % ("%dx%dx%d" % shape, f, fb, tf, tfb,
                                                                   2.0 * B * N * N * D / (f * 1e-3) / 1e12, cpu))
+    return 0
+
+
+def feature_table(only: str = None) -> int:
+    """The feature operators over the cases of perf/operators.py: time of one pass among others (32 passes between two
+    synchronisations, on three sets of inputs in turn; median of five) of the operators and of the plain forms, and the
+    bytes a pass cannot do without over the operators' time."""
+    import importlib.util
+
+    import torch
+
+    spec = importlib.util.spec_from_file_location("igs_feature_cases", os.path.join(ROOT, "perf", "operators.py"))
+    cases = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(cases)
+
+    def us(states):
+        def block(n):
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+            for i in range(n):
+                cases.run(states[i % len(states)])
+            torch.cuda.synchronize()
+            return (time.perf_counter() - t0) / n * 1e6
+
+        block(8)
+        return sorted(block(32) for _ in range(5))[2]
+
+    print("%-22s %12s %12s %10s" % ("case", "operators us", "plain us", "GB/s"))
+    for case in cases.listed():
+        if only and case["name"] != only:
+            continue
+        states = [cases.prepare(case, seed) for seed in (1, 2, 3)]
+        cases.own = True
+        own = us(states)
+        cases.own = False
+        plain = float("nan") if only else us(states)
+        print("%-22s %12.1f %12.1f %10.0f" % (case["name"], own, plain, cases.work(case)["bytes"] / own / 1e3), flush=True)
     return 0
 
 
