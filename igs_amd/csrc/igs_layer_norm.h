@@ -1,5 +1,5 @@
 // igs_layer_norm.h -- layer norm over rows, forward and backward, with dropout of its result.
-// Included by igs_feature.hip inside its anonymous namespace.
+// Included by igs_norm.hip inside its anonymous namespace.
 //
 //   h = (x - mean) rstd,  y = drop(h w + b);   d = drop(gy), g = d w
 //   gx = rstd (g - mean g - h mean(g h)),  gw = sum_rows d h,  gb = sum_rows d
