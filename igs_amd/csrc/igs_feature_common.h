@@ -1,6 +1,6 @@
 // igs_feature_common.h -- element types, wide loads, sums across lanes and the counter-based generator
 // shared by the feature operators (embedding lookup, layer norm, dropout).  Included by igs_feature.hip and
-// inside its anonymous namespace.
+// igs_norm.hip inside their anonymous namespaces.
 #pragma once
 
 constexpr int kWave = 64;

@@ -305,6 +305,12 @@ struct DropoutNode : torch::autograd::Node {
     void release_variables() override { seed_tensor.reset_data(); }
 };
 
+// Forward-mode derivatives would be dropped without a word.
+void no_tangent(const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "the feature operators have no forward-mode derivative");
+}
+
 template <class N, class... Inputs>
 std::shared_ptr<N> node_for(const Inputs&... inputs) {
     std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
@@ -314,6 +320,7 @@ std::shared_ptr<N> node_for(const Inputs&... inputs) {
 
 // ---------------------------------------------------------------------------------- differentiable operators
 Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+    no_tangent(weight);
     std::shared_ptr<EmbeddingNode> node;
     if (torch::autograd::compute_requires_grad(weight)) {
         node = node_for<EmbeddingNode>(weight);
@@ -334,6 +341,7 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64
 Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, double eps, int64_t threshold,
                   int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
     const Tensor weight = value(weight_), bias = value(bias_);
+    for (const Tensor* t : {&x, &weight, &bias}) no_tangent(*t);
     const DropoutArgs d{threshold, seed, value(seed_tensor), offset};
     std::shared_ptr<NormNode> node;
     if (torch::autograd::compute_requires_grad(x, weight, bias)) node = node_for<NormNode>(x, weight, bias);
@@ -357,6 +365,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bi
 }
 
 Tensor dropout(const Tensor& x, int64_t threshold, int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
+    no_tangent(x);
     const DropoutArgs d{threshold, seed, value(seed_tensor), offset};
     std::shared_ptr<DropoutNode> node;
     if (torch::autograd::compute_requires_grad(x)) {

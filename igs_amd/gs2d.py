@@ -332,6 +332,14 @@ class GaussianSplatting2D(nn.Module):
         a, b, d = _cov_inverse_torch(scales, rotations, eps)
         return naive_gaussian_2d(x_grid, y_grid, positions, a, b, d, alphas, colors, eps)
 
+    def __setstate__(self, state):
+        """Modules pickled whole before the front existed have none."""
+        super().__setstate__(state)
+        for name, value in (("emb_scale", 1.0), ("feature_dropout", 0.0), ("dropout_seed", None), ("embedding", None),
+                            ("norm", None)):
+            if name not in self._modules:
+                self.__dict__.setdefault(name, value)
+
     def _head_input(self, feature, fused):
         """Tokens or features -> what `proj` takes: lookup, norm and dropout where the module has them."""
         if not feature.is_floating_point():

@@ -228,6 +228,26 @@ def test_module_defaults_are_unchanged_and_options_add_parameters():
         a(torch.zeros(2, 3, dtype=torch.int64), size=(4, 4))
 
 
+def test_modules_copied_and_pickled_whole():
+    """Copies keep the front; a module pickled before there was one still runs."""
+    import copy
+    import pickle
+
+    m = igs_amd.GaussianSplatting2D(4, 16, num_embeddings=11, feature_norm=True)
+    t = torch.randint(0, 11, (2, 5))
+    want = m(t, size=(6, 7), fused=False)[0]
+    for c in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert torch.equal(c(t, size=(6, 7), fused=False)[0], want)
+    plain = igs_amd.GaussianSplatting2D(4, 16)
+    state = plain.__getstate__() if hasattr(plain, "__getstate__") else plain.__dict__
+    state = {k: v for k, v in dict(state or plain.__dict__).items()
+             if k not in ("emb_scale", "feature_dropout", "dropout_seed", "embedding", "norm")}
+    old = igs_amd.GaussianSplatting2D.__new__(igs_amd.GaussianSplatting2D)
+    old.__setstate__(state)
+    x = torch.randn(2, 5, 16)
+    assert torch.equal(old(x, size=(6, 7), fused=False)[0], plain(x, size=(6, 7), fused=False)[0])
+
+
 def test_module_debug_path_on_the_cpu():
     """fused=False: lookup, norm and dropout as plain torch, then the plain splat; the mask is the operator's."""
     torch.manual_seed(3)

@@ -586,6 +586,14 @@ def test_backward_twice_and_second_derivatives(igs, dev):
         y.sum().backward()
     with torch.inference_mode():
         assert torch.equal(igs.layer_norm(x, w), igs.layer_norm(x.clone(), w))
+    import torch.autograd.forward_ad as fwAD
+
+    with fwAD.dual_level():                              # a tangent would be lost without a word
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        for f in (lambda: igs.layer_norm(dual), lambda: igs.dropout(dual, 0.5, 1),
+                  lambda: igs.embedding_lookup(t, fwAD.make_dual(table, table))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
 
 
 def test_mixed_devices_raise(igs, dev):
