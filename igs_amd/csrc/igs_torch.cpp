@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <cmath>
 #include <optional>
 #include <tuple>
 
@@ -319,7 +320,29 @@ std::shared_ptr<N> node_for(const Inputs&... inputs) {
 }
 
 // ---------------------------------------------------------------------------------- differentiable operators
-Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+// What a caller gets wrong is refused here (a call on a small tensor takes 5 us, and each Python-level check adds to it).
+void on_gpu(const Tensor& first) {
+    TORCH_CHECK(first.device().is_cuda(), "the feature operators run on the GPU only (HIP kernels); got a tensor on ", first.device(),
+                ". The naive_* functions are the plain-torch expressions.");
+}
+void supported(const Tensor& t, const char* what) {
+    TORCH_CHECK_TYPE(dtype_code(t) >= 0, what, " must be float32, float16 or bfloat16; got ", t.scalar_type());
+}
+
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+    TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0,
+                      "weight must be [V, D] with V, D >= 1; got ", weight.sizes());
+    TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int32 or int64; got ",
+                     tokens.scalar_type());
+    supported(weight, "weight");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
+    const int64_t vocab = weight.size(0);
+    int64_t padding = padding_idx.value_or(-1);
+    if (padding_idx) {
+        TORCH_CHECK_VALUE(padding >= -vocab && padding < vocab, "padding_idx ", padding, " is outside the table of ", vocab, " rows");
+        if (padding < 0) padding += vocab;
+    }
+    on_gpu(weight);
     no_tangent(weight);
     std::shared_ptr<EmbeddingNode> node;
     if (torch::autograd::compute_requires_grad(weight)) {
@@ -340,8 +363,24 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, double eps, int64_t threshold,
                   int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
-    const Tensor weight = value(weight_), bias = value(bias_);
-    for (const Tensor* t : {&x, &weight, &bias}) no_tangent(*t);
+    TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last axis of one element or more; got ", x.sizes());
+    supported(x, "x");
+    Tensor weight = value(weight_), bias = value(bias_);
+    bool other = false;
+    for (const Tensor* t : {&weight, &bias})
+        if (t->defined()) {
+            const char* name = t == &weight ? "weight" : "bias";
+            TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(-1), name, " must be [", x.size(-1), "]; got ", t->sizes());
+            TORCH_CHECK_TYPE(t->is_floating_point(), name, " must be a floating-point tensor; got ", t->scalar_type());
+            other |= t->scalar_type() != x.scalar_type();
+        }
+    TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative; got ", eps);
+    on_gpu(x);
+    if (other) {  // weights of another type than x's are taken in fp32
+        if (weight.defined()) weight = weight.to(at::kFloat);
+        if (bias.defined()) bias = bias.to(at::kFloat);
+    }
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &weight, &bias}) no_tangent(*t);
     const DropoutArgs d{threshold, seed, value(seed_tensor), offset};
     std::shared_ptr<NormNode> node;
     if (torch::autograd::compute_requires_grad(x, weight, bias)) node = node_for<NormNode>(x, weight, bias);
@@ -365,6 +404,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bi
 }
 
 Tensor dropout(const Tensor& x, int64_t threshold, int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
+    supported(x, "x");
+    on_gpu(x);
     no_tangent(x);
     const DropoutArgs d{threshold, seed, value(seed_tensor), offset};
     std::shared_ptr<DropoutNode> node;

@@ -26,31 +26,12 @@ from . import _lib
 
 Tensor = torch.Tensor
 
-_DTYPES = {torch.float32: _lib.IGS_F32, torch.float16: _lib.IGS_F16, torch.bfloat16: _lib.IGS_BF16}
-_TOKENS = (torch.int64, torch.int32)
+_SEED_END = 1 << 63
 
 
 # --------------------------------------------------------------------------------------
 # arguments
 # --------------------------------------------------------------------------------------
-def _dtype_of(t: Tensor, what: str) -> int:
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} must be float32, float16 or bfloat16; got {t.dtype}")
-    return code
-
-
-def _on_gpu(first: Tensor, *others: Optional[Tensor]) -> None:
-    """Every tensor whose address goes to a kernel lives on one GPU: a host pointer handed to a launch
-    would be a memory fault, not an exception."""
-    if first.device.type != "cuda":
-        raise RuntimeError("the feature operators run on the GPU only (HIP kernels); got a tensor on "
-                           f"{first.device}. The naive_* functions are the plain-torch expressions.")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"Expected all tensors to be on the same device, but got {first.device} and {t.device}")
-
-
 def dropout_threshold(p: float) -> int:
     """The 16-bit limit of dropout probability p: an element is dropped if its 16-bit number is below
     it, so p acts in steps of 2^-16."""
@@ -64,8 +45,14 @@ def _seed(seed, offset, like: Tensor) -> Tuple[int, Optional[Tensor], int]:
     """(number, device tensor or None, offset): a seed is an int in [0, 2^63), or an int64 tensor of one
     element on the device, which the kernels read when they run (so a replayed graph sees its value of
     then)."""
-    if type(offset) is not int and not isinstance(offset, (int, torch.SymInt)):
+    if type(seed) is int and type(offset) is int:
+        if not (0 <= seed < _SEED_END and 0 <= offset < _SEED_END):
+            raise ValueError("seed and offset must be in [0, 2^63)")
+        return seed, None, offset
+    if not isinstance(offset, (int, torch.SymInt)) or isinstance(offset, bool):
         raise TypeError(f"offset must be an int; got {type(offset).__name__}")
+    if type(offset) is int and not 0 <= offset < _SEED_END:
+        raise ValueError("seed and offset must be in [0, 2^63)")
     if isinstance(seed, Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise TypeError("a seed tensor holds one int64 element")
@@ -77,8 +64,6 @@ def _seed(seed, offset, like: Tensor) -> Tuple[int, Optional[Tensor], int]:
         raise ValueError("dropout needs a seed (an int, or an int64 tensor of one element on the device)")
     if not isinstance(seed, (int, torch.SymInt)) or isinstance(seed, bool):
         raise TypeError(f"seed must be an int or an int64 tensor; got {type(seed).__name__}")
-    if not torch.compiler.is_compiling() and not (0 <= seed < 1 << 63 and 0 <= offset < 1 << 63):
-        raise ValueError("seed and offset must be in [0, 2^63)")
     return seed, None, offset
 
 
@@ -144,25 +129,11 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
     and rounded once; the row `padding_idx` (negative counts from the end) gets none.  A token outside
     [0, V) gives a row of NaN and reaches no gradient: nothing here waits for the device, so it cannot
     raise."""
-    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
-        raise ValueError(f"weight must be [V, D] with V, D >= 1; got {tuple(weight.shape)}")
-    if tokens.dtype not in _TOKENS:
-        raise TypeError(f"tokens must be int32 or int64; got {tokens.dtype}")
-    if weight.dtype not in _DTYPES:
-        _dtype_of(weight, "weight")
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    V = weight.shape[0]
-    if padding_idx is None:
-        padding_idx = -1
-    else:
-        if not -V <= padding_idx < V:
-            raise ValueError(f"padding_idx {padding_idx} is outside the table of {V} rows")
-        padding_idx %= V
     if torch.compiler.is_compiling():
-        return torch.ops.igs_amd.embedding_fwd(tokens, weight, scale, padding_idx)
-    _on_gpu(weight, tokens)
+        V = weight.shape[0]
+        if padding_idx is not None and not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} is outside the table of {V} rows")
+        return torch.ops.igs_amd.embedding_fwd(tokens, weight, float(scale), -1 if padding_idx is None else padding_idx % V)
     return (_torch_binding or _native()).embedding(tokens, weight, scale, padding_idx)
 
 
@@ -231,31 +202,18 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     weight, bias [D] (either may be None) in x's type or fp32; other types are converted to fp32.  Rows
     that are dense and evenly spaced are read where they are."""
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"x must have a last axis of one element or more; got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES:
-        _dtype_of(x, "x")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.dim() != 1 or t.shape[0] != x.shape[-1]:
-                raise ValueError(f"{name} must be [{x.shape[-1]}]; got {tuple(t.shape)}")
-            if not t.is_floating_point():
-                raise TypeError(f"{name} must be a floating-point tensor; got {t.dtype}")
-    if (weight is not None and weight.dtype != x.dtype) or (bias is not None and bias.dtype != x.dtype):
-        weight = weight if weight is None else weight.to(torch.float32)
-        bias = bias if bias is None else bias.to(torch.float32)
-    eps = float(eps)
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative; got {eps}")
-    threshold = dropout_threshold(dropout_p) if dropout_p else 0
-    number, seed_tensor = 0, None
-    if threshold:
-        number, seed_tensor, offset = _seed(seed, offset, x)
-    else:
+    threshold, number, seed_tensor = 0, 0, None
+    if dropout_p:
+        threshold = dropout_threshold(dropout_p)
+        if threshold:
+            number, seed_tensor, offset = _seed(seed, offset, x)
+    if not threshold:
         offset = 0
     if torch.compiler.is_compiling():
-        return torch.ops.igs_amd.layer_norm_fwd(x, weight, bias, eps, threshold, number, seed_tensor, offset)[0]
-    _on_gpu(x, weight, bias)
+        if any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
+            weight = weight if weight is None else weight.to(torch.float32)
+            bias = bias if bias is None else bias.to(torch.float32)
+        return torch.ops.igs_amd.layer_norm_fwd(x, weight, bias, float(eps), threshold, number, seed_tensor, offset)[0]
     return (_torch_binding or _native()).layer_norm(x, weight, bias, eps, threshold, number, seed_tensor, offset)
 
 
@@ -306,15 +264,12 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0) -> Tensor:
     one element on the device, read when the kernel runs: change it between replays of a captured graph
     (and not between a forward and its backward).  Calls of one step that must differ take different
     offsets.  A dropped element is 0 also where x is NaN or infinite."""
-    if x.dtype not in _DTYPES:
-        _dtype_of(x, "x")
     threshold = dropout_threshold(p)
     if threshold == 0:
         return x
     number, seed_tensor, offset = _seed(seed, offset, x)
     if torch.compiler.is_compiling():
         return torch.ops.igs_amd.dropout(x, threshold, number, seed_tensor, offset)
-    _on_gpu(x)
     return (_torch_binding or _native()).dropout(x, threshold, number, seed_tensor, offset)
 
 
