@@ -596,6 +596,40 @@ def test_backward_twice_and_second_derivatives(igs, dev):
                 f()
 
 
+def test_function_transforms_and_fake_tensors_raise(igs, dev):
+    """torch.func's wrappers and fake tensors hold no memory that a kernel could read: refused, never a wrong result."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, t, table = torch.randn(5, 8, device=dev), torch.tensor([1, 2, 2], device=dev), torch.randn(4, 8, device=dev)
+    for f, leaf in ((lambda v: igs.embedding_lookup(t, v), table), (igs.layer_norm, x), (lambda v: igs.dropout(v, 0.5, 1), x)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.grad(lambda v: f(v).sum())(leaf)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.vmap(f)(leaf.expand(3, *leaf.shape))
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises((RuntimeError, NotImplementedError)):
+            f(torch.empty(4, 8, device=dev))
+    assert torch.equal(igs.embedding_lookup(t, table), table[t])
+
+
+def test_checkpointed_module_draws_the_same_mask_again(igs, dev):
+    """The module draws its dropout seed on the device from torch's generator, whose state a checkpoint restores for the
+    recomputation (of the devices of its tensor arguments): gradients are bit-equal to those of the plain step from the
+    same generator state."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(4)
+    m = igs.GaussianSplatting2D(8, 64, num_embeddings=30, feature_norm=True, feature_dropout=0.4).to(dev)
+    t = torch.randint(0, 30, (2, 16), device=dev)
+    res = []
+    for run in (lambda: m(t, size=(12, 16))[0], lambda: checkpoint(lambda a: m(a, size=(12, 16))[0], t, use_reentrant=False)):
+        m.zero_grad()
+        torch.manual_seed(7)
+        img = run()
+        img.square().sum().backward()
+        res.append([img.detach()] + [p.grad.clone() for p in m.parameters()])
+    assert len(res[0]) == len(res[1]) and all(torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_mixed_devices_raise(igs, dev):
     w, t, x = torch.randn(5, 4, device=dev), torch.tensor([1]), torch.randn(3, 4, device=dev)
     with pytest.raises(RuntimeError, match="same device"):
