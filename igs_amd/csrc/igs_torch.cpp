@@ -61,14 +61,15 @@ void check(int rc, const char* what) {
     TORCH_CHECK(rc == 0, what, " failed: ", lib.status_string(rc), " (status ", rc, ")");
 }
 
-int dtype_code(const Tensor& t) {
-    switch (t.scalar_type()) {
+int dtype_code(at::ScalarType type) {
+    switch (type) {
         case at::kFloat: return IGS_F32;
         case at::kHalf: return IGS_F16;
         case at::kBFloat16: return IGS_BF16;
         default: return -1;  // the library refuses it
     }
 }
+int dtype_code(const Tensor& t) { return dtype_code(t.scalar_type()); }
 
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* writable(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -208,7 +209,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
     const Tensor gx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor gw = want_w ? at::empty({D}, wopts) : Tensor(), gb = want_b ? at::empty({D}, wopts) : Tensor();
     const int code = dtype_code(x);
-    const int wcode = wtype == at::kFloat ? IGS_F32 : wtype == at::kHalf ? IGS_F16 : IGS_BF16;
+    const int wcode = dtype_code(wtype);
     igs_layer_norm_plan_t plan;
     check(lib.layer_norm_plan(rows, width(D), code, wcode, &plan), "igs_layer_norm_plan");
     const Tensor ws = workspace(plan.ws_bytes, x);
@@ -447,6 +448,7 @@ PYBIND11_MODULE(_igs_torch, m) {
         [](const Tensor& grad, const Tensor& x, const OptTensor& w, const OptTensor& b, const Tensor& stats,
            int64_t threshold, int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
             const Tensor weight = value(w), bias = value(b);
+            check_weights(x, weight, bias);
             auto [gx, gw, gb] = norm_bwd(grad, x, weight, (w ? weight : b ? bias : x).scalar_type(), stats,
                                          DropoutArgs{threshold, seed, value(seed_tensor), offset}, true, w.has_value(), b.has_value());
             std::vector<Tensor> out{gx};

@@ -268,3 +268,32 @@ def test_module_debug_path_on_the_cpu():
     torch.manual_seed(5)
     assert torch.equal(a, m(t, size=(6, 7), fused=False)[1])                                        # torch's generator governs it
     m(torch.randn(2, 5, 16), size=(6, 7), fused=False)   # features still pass
+
+
+# ---------------------------------------------------------------------------------- direct calls below the public functions
+def norm_bwd_arguments(dtype=torch.bfloat16, D=16, rows=3):
+    x = torch.randn(rows, D).to(dtype)
+    return torch.randn(rows, D).to(dtype), x, torch.zeros(rows, 2)
+
+
+@pytest.mark.parametrize("wtype", [torch.int8, torch.uint8, torch.bool, torch.int64, torch.float64, torch.float16], ids=str)
+def test_norm_backward_refuses_weights_of_other_types(wtype):
+    """Weight or bias alone, of a type that the kernels would read and write as another: refused by the library's own check,
+    before anything is launched (so without a GPU too)."""
+    grad, x, stats = norm_bwd_arguments()
+    w = torch.ones(16).to(wtype)
+    bwd = feature._native().layer_norm_bwd
+    for weight, bias in ((w, None), (None, w), (w, w)):
+        with pytest.raises(RuntimeError, match="element type"):
+            bwd(grad, x, weight, bias, stats, 0, 0, None, 0)
+
+
+def test_norm_backward_refuses_a_bias_that_does_not_fit():
+    """A bias of another type or length than the weight's beside a good weight (its gradient would be the weight's)."""
+    grad, x, stats = norm_bwd_arguments()
+    w = torch.ones(16)
+    bwd = feature._native().layer_norm_bwd
+    with pytest.raises(RuntimeError, match="one type"):
+        bwd(grad, x, w, w.bfloat16(), stats, 0, 0, None, 0)
+    with pytest.raises(RuntimeError, match="must be"):
+        bwd(grad, x, w, torch.ones(15), stats, 0, 0, None, 0)
