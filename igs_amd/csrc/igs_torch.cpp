@@ -165,6 +165,7 @@ struct DropoutArgs {
     Tensor seed_tensor;
     int64_t offset;
     void check(const Tensor& x) const {
+        TORCH_CHECK(threshold >= 0 && threshold <= 65536, "a dropout threshold is in 0..65536; got ", threshold);  // 64 bits here
         same_device(x, seed_tensor, "the seed");
         TORCH_CHECK(!seed_tensor.defined() || (seed_tensor.scalar_type() == at::kLong && seed_tensor.numel() == 1),
                     "a seed tensor holds one int64 element");

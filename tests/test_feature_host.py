@@ -297,3 +297,15 @@ def test_norm_backward_refuses_a_bias_that_does_not_fit():
         bwd(grad, x, w, w.bfloat16(), stats, 0, 0, None, 0)
     with pytest.raises(RuntimeError, match="must be"):
         bwd(grad, x, w, torch.ones(15), stats, 0, 0, None, 0)
+
+
+@pytest.mark.parametrize("threshold", [-1, 65537, 1 << 32, (1 << 32) + 100, -(1 << 32)])
+def test_thresholds_are_checked_in_64_bits(threshold):
+    """One whose lower 32 bits are a good threshold (2^32: no dropout) is refused like any other outside 0..65536."""
+    native, x = feature._native(), torch.randn(3, 16)
+    grad, xb, stats = norm_bwd_arguments()
+    for call in (lambda: native.dropout_plain(x, threshold, 1, None, 0),
+                 lambda: native.layer_norm_fwd(x, None, None, 1e-5, threshold, 1, None, 0),
+                 lambda: native.layer_norm_bwd(grad, xb, None, None, stats, threshold, 1, None, 0)):
+        with pytest.raises(RuntimeError, match="threshold is in 0..65536"):
+            call()
