@@ -8,13 +8,16 @@
 // but resolved from the handle that the ctypes binding has open, so both use the same one.
 #include <torch/extension.h>
 
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
@@ -233,6 +236,48 @@ Tensor dropout_call(const Tensor& x_, const DropoutArgs& d) {
     return y;
 }
 
+// ---------------------------------------------------------------------------------- tracers and dispatch modes
+// torch.jit.trace and make_fx record the operators that torch dispatches, and a dispatch mode may replace them.  Of the
+// calls here they see the allocation of the result and nothing else: a traced function would return memory that nothing
+// wrote.  The registered operators are taken then: by the caller in Python where a differentiable operator returns
+// nothing, and in the nodes below for a backward of what was called before.
+bool dispatch_mode() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+bool recorded() { return torch::jit::tracer::isTracing() || dispatch_mode(); }
+
+// Fake tensors and other subclasses hold no memory, and the operators have no rule for them.
+void plain_tensors(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->key_set().has(c10::DispatchKey::Python),
+                                    "the feature operators take plain tensors; got a fake tensor or another subclass "
+                                    "(under torch.compile and torch.export they are registered operators)");
+}
+
+template <class F>
+c10::TypedOperatorHandle<F> registered(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+Tensor embedding_bwd_recorded(const Tensor& grad, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+    return registered<Tensor(const Tensor&, const Tensor&, c10::SymInt, double, c10::SymInt)>("igs_amd::embedding_bwd")
+        .call(grad, tokens, vocab, scale, padding);
+}
+variable_list norm_bwd_recorded(const Tensor& grad, const Tensor& x, const Tensor& weight, at::ScalarType wtype,
+                                const Tensor& stats, const DropoutArgs& d, bool want_w, bool want_b) {
+    // of the bias the operator takes the type and the length alone
+    const Tensor bias = !want_b ? Tensor() : weight.defined() ? weight : at::empty({x.size(-1)}, x.options().dtype(wtype));
+    const std::vector<Tensor> g =
+        registered<std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&, c10::SymInt,
+                                       c10::SymInt, const OptTensor&, c10::SymInt)>("igs_amd::layer_norm_bwd")
+            .call(grad, x, optional(weight), optional(bias), stats, d.threshold, d.seed, optional(d.seed_tensor), d.offset);
+    const size_t at_b = weight.defined() ? 2 : 1;
+    return {g[0], want_w ? g[1] : Tensor(), want_b ? g[at_b] : Tensor()};
+}
+Tensor dropout_recorded(const Tensor& x, const DropoutArgs& d) {
+    return registered<Tensor(const Tensor&, c10::SymInt, c10::SymInt, const OptTensor&, c10::SymInt)>("igs_amd::dropout")
+        .call(x, d.threshold, d.seed, optional(d.seed_tensor), d.offset);
+}
+
 // ---------------------------------------------------------------------------------- autograd nodes
 // Gradients as the engine gets them.  The nodes differentiate once: where the backward is itself being recorded
 // (create_graph), what it returns raises when it is differentiated.
@@ -257,7 +302,7 @@ struct EmbeddingNode : torch::autograd::Node {
         Tensor g;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            g = embedding_bwd(grads[0], t, vocab, scale, padding);
+            g = (dispatch_mode() ? embedding_bwd_recorded : embedding_bwd)(grads[0], t, vocab, scale, padding);
         }
         return once({g}, grads[0].requires_grad());
     }
@@ -278,7 +323,8 @@ struct NormNode : torch::autograd::Node {
         variable_list out(3);
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            std::tie(out[0], out[1], out[2]) = norm_bwd(grads[0], xs, ws, wtype, st, d, need[0], need[1], need[2]);
+            if (dispatch_mode()) out = norm_bwd_recorded(grads[0], xs, ws, wtype, st, d, need[1], need[2]);
+            else std::tie(out[0], out[1], out[2]) = norm_bwd(grads[0], xs, ws, wtype, st, d, need[0], need[1], need[2]);
         }
         return once(std::move(out), grads[0].requires_grad() || xs.requires_grad() || (ws.defined() && ws.requires_grad()));
     }
@@ -301,7 +347,7 @@ struct DropoutNode : torch::autograd::Node {
         Tensor g;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            g = dropout_call(grads[0], d);
+            g = (dispatch_mode() ? dropout_recorded : dropout_call)(grads[0], d);
         }
         return once({g}, grads[0].requires_grad());
     }
@@ -331,21 +377,26 @@ void supported(const Tensor& t, const char* what) {
     TORCH_CHECK_TYPE(dtype_code(t) >= 0, what, " must be float32, float16 or bfloat16; got ", t.scalar_type());
 }
 
-Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+// The row of padding_idx, which may count from the end of the table (-1: none).
+int64_t padding_row(const Tensor& weight, std::optional<int64_t> padding_idx) {
+    if (!padding_idx) return -1;
+    const int64_t vocab = weight.size(0), row = *padding_idx;
+    TORCH_CHECK_VALUE(row >= -vocab && row < vocab, "padding_idx ", row, " is outside the table of ", vocab, " rows");
+    return row < 0 ? row + vocab : row;
+}
+
+// These return nothing under a tracer or a dispatch mode: the caller takes the registered operator.
+OptTensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
     TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0,
                       "weight must be [V, D] with V, D >= 1; got ", weight.sizes());
     TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int32 or int64; got ",
                      tokens.scalar_type());
     supported(weight, "weight");
     TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
-    const int64_t vocab = weight.size(0);
-    int64_t padding = padding_idx.value_or(-1);
-    if (padding_idx) {
-        TORCH_CHECK_VALUE(padding >= -vocab && padding < vocab, "padding_idx ", padding, " is outside the table of ", vocab, " rows");
-        if (padding < 0) padding += vocab;
-    }
+    const int64_t padding = padding_row(weight, padding_idx);
     on_gpu(weight);
     no_tangent(weight);
+    if (recorded()) return plain_tensors({&tokens, &weight}), OptTensor();
     std::shared_ptr<EmbeddingNode> node;
     if (torch::autograd::compute_requires_grad(weight)) {
         node = node_for<EmbeddingNode>(weight);
@@ -363,8 +414,8 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::
     return y;
 }
 
-Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, double eps, int64_t threshold,
-                  int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
+OptTensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, double eps, int64_t threshold,
+                     int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last axis of one element or more; got ", x.sizes());
     supported(x, "x");
     Tensor weight = value(weight_), bias = value(bias_);
@@ -378,6 +429,10 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bi
         }
     TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative; got ", eps);
     on_gpu(x);
+    if (recorded()) {
+        for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &weight, &bias}) no_tangent(*t);
+        return plain_tensors({&x, &weight, &bias}), OptTensor();
+    }
     if (other) {  // weights of another type than x's are taken in fp32
         if (weight.defined()) weight = weight.to(at::kFloat);
         if (bias.defined()) bias = bias.to(at::kFloat);
@@ -405,10 +460,11 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bi
     return y;
 }
 
-Tensor dropout(const Tensor& x, int64_t threshold, int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
+OptTensor dropout(const Tensor& x, int64_t threshold, int64_t seed, const OptTensor& seed_tensor, int64_t offset) {
     supported(x, "x");
     on_gpu(x);
     no_tangent(x);
+    if (recorded()) return plain_tensors({&x}), OptTensor();
     const DropoutArgs d{threshold, seed, value(seed_tensor), offset};
     std::shared_ptr<DropoutNode> node;
     if (torch::autograd::compute_requires_grad(x)) {
@@ -434,7 +490,8 @@ PYBIND11_MODULE(_igs_torch, m) {
     m.def("embedding", &embedding, nogil);
     m.def("layer_norm", &layer_norm, nogil);
     m.def("dropout", &dropout, nogil);
-    // without autograd, for the registered operators of torch.compile
+    m.def("padding_row", &padding_row);
+    // without autograd, for the registered operators
     m.def("embedding_fwd", &embedding_fwd, nogil);
     m.def("embedding_bwd", &embedding_bwd, nogil);
     m.def(

@@ -10,8 +10,9 @@ operators that make such a feature out of token ids or of a trunk's output, forw
 `GaussianSplatting2D` calls them when it is built with `num_embeddings=`, `feature_norm=` or
 `feature_dropout=`.  fp32, fp16 and bf16; sums and norms are held in fp32 and every result is rounded
 once; gradients of weights are summed in a fixed order (bit-reproducible).  Eager callers go through
-native autograd nodes (csrc/igs_torch.cpp) around the C ABI; under `torch.compile` the same library
-calls are registered operators (`igs_amd::embedding_fwd` and its like).  There is no CPU path: tensors must live on the GPU.  The
+native autograd nodes (csrc/igs_torch.cpp) around the C ABI; under `torch.compile`, `torch.export`,
+`torch.jit.trace`, `make_fx` and other dispatch modes the same library calls are registered operators
+(`igs_amd::embedding_fwd` and its like).  There is no CPU path: tensors must live on the GPU.  The
 `naive_*` functions are the plain torch expressions (any device), what the module's `fused=False`
 debug path uses.
 """
@@ -134,7 +135,11 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
         if padding_idx is not None and not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} is outside the table of {V} rows")
         return torch.ops.igs_amd.embedding_fwd(tokens, weight, float(scale), -1 if padding_idx is None else padding_idx % V)
-    return (_torch_binding or _native()).embedding(tokens, weight, scale, padding_idx)
+    native = _torch_binding or _native()
+    y = native.embedding(tokens, weight, scale, padding_idx)
+    if y is None:   # something records the operators
+        y = torch.ops.igs_amd.embedding_fwd(tokens, weight, float(scale), native.padding_row(weight, padding_idx))
+    return y
 
 
 def naive_embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
@@ -209,12 +214,14 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
             number, seed_tensor, offset = _seed(seed, offset, x)
     if not threshold:
         offset = 0
-    if torch.compiler.is_compiling():
-        if any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
-            weight = weight if weight is None else weight.to(torch.float32)
-            bias = bias if bias is None else bias.to(torch.float32)
-        return torch.ops.igs_amd.layer_norm_fwd(x, weight, bias, float(eps), threshold, number, seed_tensor, offset)[0]
-    return (_torch_binding or _native()).layer_norm(x, weight, bias, eps, threshold, number, seed_tensor, offset)
+    if not torch.compiler.is_compiling():
+        y = (_torch_binding or _native()).layer_norm(x, weight, bias, eps, threshold, number, seed_tensor, offset)
+        if y is not None:   # else something records the operators
+            return y
+    if any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
+        weight = weight if weight is None else weight.to(torch.float32)
+        bias = bias if bias is None else bias.to(torch.float32)
+    return torch.ops.igs_amd.layer_norm_fwd(x, weight, bias, float(eps), threshold, number, seed_tensor, offset)[0]
 
 
 def naive_layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -268,9 +275,11 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0) -> Tensor:
     if threshold == 0:
         return x
     number, seed_tensor, offset = _seed(seed, offset, x)
-    if torch.compiler.is_compiling():
-        return torch.ops.igs_amd.dropout(x, threshold, number, seed_tensor, offset)
-    return (_torch_binding or _native()).dropout(x, threshold, number, seed_tensor, offset)
+    if not torch.compiler.is_compiling():
+        y = (_torch_binding or _native()).dropout(x, threshold, number, seed_tensor, offset)
+        if y is not None:   # else something records the operators
+            return y
+    return torch.ops.igs_amd.dropout(x, threshold, number, seed_tensor, offset)
 
 
 def _mul32(a: int, b: Tensor) -> Tuple[Tensor, Tensor]:

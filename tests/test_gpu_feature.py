@@ -727,3 +727,95 @@ def test_compiled_operators(igs, dev):
     m.dropout_seed = None                                # a seed drawn on the device inside the graph
     torch.compile(lambda v: m(v, size=(9, 11)), fullgraph=True)(ids)[0].sum().backward()
     assert bool(m.embedding.weight.grad.isfinite().all()) and bool(m.embedding.weight.grad.any())
+
+
+# ---------------------------------------------------------------------------------- tracers and dispatch modes
+def traced_chain(igs, t, seed):
+    """tokens and weights -> features, with every operator and with weights of another type than the rows'."""
+    def fn(w, gw, gb):
+        f = igs.layer_norm(igs.embedding_lookup(t, w, 1.5, -2), gw, gb, dropout_p=0.2, seed=seed, offset=1)
+        return igs.dropout(igs.layer_norm(f, gw.bfloat16()), 0.1, seed, 5)
+    return fn
+
+
+def traced_inputs(dev, first):
+    V, D = 40, 72
+    return [normal(s, first + i, torch.float32, m).to(dev) for i, (s, m) in enumerate((((V, D), 0.0), ((D,), 1.0), ((D,), 0.0)))]
+
+
+@pytest.mark.parametrize("tensor_seed", [False, True])
+@pytest.mark.parametrize("how", ["jit", "fx"])
+def test_traced_functions_compute_the_operators(igs, dev, how, tensor_seed):
+    """A trace records the registered operators: on other inputs than it was made with it gives the eager results, forward
+    and (a traced graph being differentiable) backward."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    t = some_tokens(50, 40, 1, "skew").to(dev)
+    fn = traced_chain(igs, t, torch.tensor([31], device=dev) if tensor_seed else 31)
+    trace = make_fx(fn) if how == "fx" else None
+    traced = trace(*traced_inputs(dev, 1)) if how == "fx" else torch.jit.trace(fn, tuple(traced_inputs(dev, 1)))
+    up = normal((50, 72), 9, torch.float32).to(dev)
+    res = []
+    for f in (fn, traced):
+        lv = [v.requires_grad_(True) for v in traced_inputs(dev, 20)]
+        y = f(*lv)
+        res.append((y.detach(), *torch.autograd.grad(y, lv, up)))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
+def test_traced_gradients_compute_the_operators(igs, dev):
+    """make_fx of a gradient: of a function traced whole, and of one that was called before the trace began."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    t = some_tokens(50, 40, 1, "skew").to(dev)
+    fn = traced_chain(igs, t, 31)
+    lv = [v.requires_grad_(True) for v in traced_inputs(dev, 1)]
+    first, up = normal((50, 72), 8, torch.float32).to(dev), normal((50, 72), 9, torch.float32).to(dev)
+    whole = lambda w, gw, gb, g: torch.autograd.grad(fn(w, gw, gb), (w, gw, gb), g)
+    other = [v.requires_grad_(True) for v in traced_inputs(dev, 20)]
+    for a, b in zip(make_fx(whole)(*lv, first)(*other, up), whole(*other, up)):
+        assert torch.equal(a, b)
+    y = fn(*lv)
+    want = torch.autograd.grad(y, lv, up, retain_graph=True)
+    later = make_fx(lambda g: torch.autograd.grad(y, lv, g, retain_graph=True))(first)
+    for a, b in zip(later(up), want):
+        assert torch.equal(a, b)
+    example = first.clone()                              # (a trace replaces its example wherever it meets it: not the norm's x)
+    for which in range(3):                               # a part of the inputs alone
+        w = igs.layer_norm(first, lv[1], lv[2]) if which else igs.embedding_lookup(t, lv[0])
+        (want,) = torch.autograd.grad(w, lv[which], up, retain_graph=True)
+        (got,) = make_fx(lambda g: torch.autograd.grad(w, lv[which], g, retain_graph=True))(example)(up)
+        assert torch.equal(got, want)
+    b = igs.layer_norm(first, None, lv[2])               # a bias without a weight
+    (got,) = make_fx(lambda g: torch.autograd.grad(b, lv[2], g, retain_graph=True))(example)(up)
+    assert torch.equal(got, torch.autograd.grad(b, lv[2], up)[0])
+
+
+def test_dispatch_modes_see_the_operators(igs, dev):
+    """A mode that counts what is dispatched sees one operator per call, forward and backward, and the results stay."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    t = some_tokens(50, 40, 1, "skew").to(dev)
+    fn = traced_chain(igs, t, 31)
+    lv, up = [v.requires_grad_(True) for v in traced_inputs(dev, 1)], normal((50, 72), 9, torch.float32).to(dev)
+    y = fn(*lv)
+    want = torch.autograd.grad(y, lv, up, retain_graph=True)
+    with Count() as c:
+        assert torch.equal(fn(*lv).detach(), y.detach())
+    ours = [n for n in c.seen if n.startswith("igs_amd::")]
+    assert ours == ["igs_amd::embedding_fwd", "igs_amd::layer_norm_fwd", "igs_amd::layer_norm_fwd", "igs_amd::dropout"], ours
+    with Count() as c:
+        got = torch.autograd.grad(y, lv, up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ours = [n for n in c.seen if n.startswith("igs_amd::")]
+    assert ours == ["igs_amd::dropout", "igs_amd::layer_norm_bwd", "igs_amd::layer_norm_bwd", "igs_amd::embedding_bwd"], ours
