@@ -87,10 +87,15 @@ Tensor workspace(uint64_t bytes, const Tensor& like) {
     return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// What the kernels read are a tensor's bytes: a negation that is yet to be done (the imaginary part of a conjugate) is
+// done first.  contiguous() leaves it where it copies nothing.
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous().resolve_neg() : t; }
+
 // (x or a contiguous copy, distance of its rows in elements): rows of the last axis are taken where they are if they
 // are dense and evenly spaced (slices of the last axis, expanded batches).
 std::tuple<Tensor, int64_t> rows_of(const Tensor& x) {
     const int64_t D = x.size(-1);
+    if (x.is_neg()) return {dense(x), D};
     if (x.is_contiguous()) return {x, D};
     if (D != 1 && x.stride(-1) != 1) return {x.contiguous(), D};
     int64_t step = -1, span = -1;
@@ -132,9 +137,9 @@ Tensor embedding_fwd(const Tensor& tokens_, const Tensor& weight_, double scale)
     check_tokens(tokens_);
     same_device(weight_, tokens_, "tokens");
     TORCH_CHECK(weight_.dim() == 2, "weight must be [V, D]");
-    const Tensor tokens = tokens_.contiguous();
+    const Tensor tokens = dense(tokens_);
     const int64_t vocab = weight_.size(0), D = weight_.size(1);
-    const Tensor weight = D > 1 && weight_.stride(1) != 1 ? weight_.contiguous() : weight_;
+    const Tensor weight = weight_.is_neg() || (D > 1 && weight_.stride(1) != 1) ? dense(weight_) : weight_;
     at::DimVector shape(tokens.sizes());
     shape.push_back(D);
     const Tensor out = at::empty(shape, weight.options());
@@ -150,7 +155,7 @@ Tensor embedding_bwd(const Tensor& grad_, const Tensor& tokens_, int64_t vocab, 
     check_tokens(tokens_);
     same_device(grad_, tokens_, "tokens");
     TORCH_CHECK(grad_.dim() > 0 && grad_.numel() == tokens_.numel() * grad_.size(-1), "one gradient row per token");
-    const Tensor grad = grad_.contiguous(), tokens = tokens_.contiguous();
+    const Tensor grad = dense(grad_), tokens = dense(tokens_);
     const int64_t D = grad.size(-1), n = tokens.numel();
     const int code = dtype_code(grad);
     igs_embedding_plan_t plan;
@@ -170,7 +175,7 @@ struct DropoutArgs {
     void check(const Tensor& x) const {
         TORCH_CHECK(threshold >= 0 && threshold <= 65536, "a dropout threshold is in 0..65536; got ", threshold);  // 64 bits here
         same_device(x, seed_tensor, "the seed");
-        TORCH_CHECK(!seed_tensor.defined() || (seed_tensor.scalar_type() == at::kLong && seed_tensor.numel() == 1),
+        TORCH_CHECK(!seed_tensor.defined() || (seed_tensor.scalar_type() == at::kLong && seed_tensor.numel() == 1 && !seed_tensor.is_neg()),
                     "a seed tensor holds one int64 element");
     }
 };
@@ -182,7 +187,7 @@ std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x_, const Tensor& weight_, con
     check_weights(x_, weight_, bias_);
     d.check(x_);
     const auto [x, step] = rows_of(x_);
-    const Tensor weight = weight_.defined() ? weight_.contiguous() : weight_, bias = bias_.defined() ? bias_.contiguous() : bias_;
+    const Tensor weight = dense(weight_), bias = dense(bias_);
     const int64_t D = x.size(-1), rows = x.numel() / D;
     const Tensor y = at::empty(x.sizes(), x.options());
     const Tensor stats = want_stats ? at::empty({rows, 2}, x.options().dtype(at::kFloat)) : Tensor();
@@ -207,7 +212,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
     TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * (x_.numel() / x_.size(-1)),
                 "the statistics are the forward's");
     const auto [x, step] = rows_of(x_);
-    const Tensor grad = grad_.contiguous(), weight = weight_.defined() ? weight_.contiguous() : weight_;
+    const Tensor grad = dense(grad_), weight = dense(weight_);
     const int64_t D = x.size(-1), rows = x.numel() / D;
     const auto wopts = x.options().dtype(wtype);
     const Tensor gx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
@@ -229,7 +234,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& grad_, const Tensor& x
 Tensor dropout_call(const Tensor& x_, const DropoutArgs& d) {
     const c10::OptionalDeviceGuard guard(x_.device());
     d.check(x_);
-    const Tensor x = x_.contiguous(), y = at::empty(x.sizes(), x.options());
+    const Tensor x = dense(x_), y = at::empty(x.sizes(), x.options());
     check(lib.dropout(address(x), dtype_code(x), x.numel(), static_cast<int>(d.threshold), static_cast<uint64_t>(d.seed),
                       seed_address(d.seed_tensor), static_cast<uint64_t>(d.offset), writable(y), stream_of(x)),
           "igs_dropout");

@@ -309,3 +309,13 @@ def test_thresholds_are_checked_in_64_bits(threshold):
                  lambda: native.layer_norm_bwd(grad, xb, None, None, stats, threshold, 1, None, 0)):
         with pytest.raises(RuntimeError, match="threshold is in 0..65536"):
             call()
+
+
+def test_rows_of_a_negative_view():
+    """A lazily negated tensor (the imaginary part of a conjugate) has the other sign in memory: it is copied."""
+    x = torch.randn(5, 6)
+    rows, step = feature._native().rows_of(torch._neg_view(x))
+    assert not rows.is_neg() and step == 6 and torch.equal(rows, -x)
+    z = torch.randn(5, 1, dtype=torch.complex64)
+    rows, step = feature._native().rows_of(z.conj().imag)
+    assert not rows.is_neg() and step == 1 and torch.equal(rows, -z.imag)

@@ -819,3 +819,37 @@ def test_dispatch_modes_see_the_operators(igs, dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     ours = [n for n in c.seen if n.startswith("igs_amd::")]
     assert ours == ["igs_amd::dropout", "igs_amd::layer_norm_bwd", "igs_amd::layer_norm_bwd", "igs_amd::embedding_bwd"], ours
+
+
+def test_lazily_negated_tensors(igs, dev):
+    """Tensors whose negation is yet to be done (the imaginary part of a conjugate), as every argument of every operator and
+    as the upstream gradient, give what the negated copies give."""
+    z = torch.view_as_complex(normal((9, 1, 2), 1, torch.float32).to(dev))
+    t = torch.tensor([3, 8, 3, 0], device=dev)
+    neg = torch._neg_view
+    x, w, b, table, up = [normal(s, i, torch.float32, 1.0).to(dev) for i, s in enumerate(((6, 24), (24,), (24,), (9, 24), (6, 24)))]
+    for lazy in (z.conj().imag, neg(table), neg(table)[:, :7], neg(table).t()):
+        assert lazy.is_neg()
+        assert torch.equal(igs.embedding_lookup(t, lazy), lazy.clone().resolve_neg()[t])
+    assert torch.equal(igs.embedding_lookup(neg(-t), table), table[t])
+    for lazy in (z.conj().imag, z.conj().imag[:1], neg(x), neg(x)[:, 3:], neg(x).t()):
+        done = lazy.resolve_neg()
+        assert lazy.is_neg() and not done.is_neg()
+        assert torch.equal(igs.dropout(lazy, 0.3, 5), igs.dropout(done, 0.3, 5))
+        assert torch.equal(igs.layer_norm(lazy), igs.layer_norm(done))
+    res = []
+    for f in (neg, torch.neg):
+        lv = [f(v).detach().requires_grad_(True) for v in (x, w, b, table)]
+        assert lv[0].is_neg() == (f is neg)
+        y = igs.dropout(igs.layer_norm(lv[0], lv[1], lv[2]), 0.3, 5)
+        e = igs.embedding_lookup(t, lv[3], 2.0)
+        res.append((y.detach(), e.detach(), *torch.autograd.grad(y, lv[:3], f(up)), *torch.autograd.grad(e, lv[3], f(up)[:4])))
+    for a, c in zip(*res):
+        assert torch.equal(a, c)
+    for node in (lambda v: igs.dropout(v, 0.3, 5), igs.layer_norm, lambda v: igs.embedding_lookup(t[:1], v)):
+        leaf = z.real.clone().requires_grad_(True)       # one element: contiguous whatever its strides
+        y = node(leaf)
+        g = z.conj().imag[:y.shape[0]]
+        assert g.is_neg() and torch.equal(*[torch.autograd.grad(y, leaf, v, retain_graph=True)[0] for v in (g, g.resolve_neg())])
+    with pytest.raises(RuntimeError, match="seed"):
+        igs.dropout(x, 0.3, neg(torch.tensor([5], device=dev)))
