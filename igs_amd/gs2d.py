@@ -295,6 +295,7 @@ class GaussianSplatting2D(nn.Module):
         self.feature_dropout = float(feature_dropout)
         self.dropout_seed = None
         self.embedding = None if num_embeddings is None else nn.Embedding(num_embeddings, emb_dim, padding_idx)
+        self._feature_norm = bool(feature_norm)   # a subclass may have a `norm` of its own
         self.norm = nn.LayerNorm(emb_dim) if feature_norm else None
 
     @staticmethod
@@ -333,12 +334,21 @@ class GaussianSplatting2D(nn.Module):
         return naive_gaussian_2d(x_grid, y_grid, positions, a, b, d, alphas, colors, eps)
 
     def __setstate__(self, state):
-        """Modules pickled whole before the front existed have none."""
+        """Modules pickled whole before the front existed have none; later ones have a norm where `norm` is not None."""
         super().__setstate__(state)
+        if "_feature_norm" not in self.__dict__:
+            self._feature_norm = "emb_scale" in self.__dict__ and getattr(self, "norm", None) is not None
         for name, value in (("emb_scale", 1.0), ("feature_dropout", 0.0), ("dropout_seed", None), ("embedding", None),
                             ("norm", None)):
             if name not in self._modules:
                 self.__dict__.setdefault(name, value)
+
+    def _has_norm(self):
+        return self._feature_norm and self.norm is not None
+
+    def _dropout_p(self):
+        """`feature_dropout`, unless a subclass has a module of that name."""
+        return self.feature_dropout if isinstance(self.feature_dropout, (int, float)) else 0.0
 
     def _head_input(self, feature, fused):
         """Tokens or features -> what `proj` takes: lookup, norm and dropout where the module has them."""
@@ -347,11 +357,11 @@ class GaussianSplatting2D(nn.Module):
                 raise TypeError(f"feature must be floating point (the module has no embedding table); got {feature.dtype}")
             lookup = _feature.embedding_lookup if fused else _feature.naive_embedding_lookup
             feature = lookup(feature, self.embedding.weight, self.emb_scale, self.embedding.padding_idx)
-        p = self.feature_dropout if self.training else 0.0
+        p = self._dropout_p() if self.training else 0.0
         seed = self.dropout_seed
         if p and seed is None:
             seed = torch.randint(0x7FFFFFFFFFFFFFFF, (1,), dtype=torch.int64, device=feature.device)
-        if self.norm is not None:
+        if self._has_norm():
             norm = _feature.layer_norm if fused else _feature.naive_layer_norm
             return norm(feature, self.norm.weight, self.norm.bias, self.norm.eps, p, seed)
         if p:
@@ -361,7 +371,7 @@ class GaussianSplatting2D(nn.Module):
     def forward(self, feature, size=None, grid=None, pos_map=None, eps=1e-6, fused=True, scale=None):
         """feature [B,F,D], or token ids [B,F] where the module has a table -> (image [B,C,H,W],
         gs_feature [B,F*n,6+C]) (src/igs/gs2d.py:611-689)."""
-        if self.norm is not None or self.feature_dropout or not feature.is_floating_point():
+        if self._has_norm() or self._dropout_p() or not feature.is_floating_point():
             feature = self._head_input(feature, fused)
         gs_feature = self.proj(feature).unflatten(-1, (-1, 6 + self.output_dim)).flatten(1, 2)
         b = gs_feature.shape[0]

@@ -319,3 +319,38 @@ def test_rows_of_a_negative_view():
     z = torch.randn(5, 1, dtype=torch.complex64)
     rows, step = feature._native().rows_of(z.conj().imag)
     assert not rows.is_neg() and step == 1 and torch.equal(rows, -z.imag)
+
+
+def test_subclasses_with_a_norm_of_their_own():
+    """A subclass that has submodules called `norm` and `feature_dropout` and applies them itself, written when the module
+    had none: the module's forward leaves them alone, built, copied and unpickled."""
+    import copy
+
+    class Own(igs_amd.GaussianSplatting2D):
+        def __init__(self):
+            super().__init__(4, 16)
+            self.norm, self.feature_dropout, self.feature_norm = torch.nn.Tanh(), torch.nn.Dropout(0.0), torch.nn.Identity()
+
+        def forward(self, feature, **kw):
+            return super().forward(self.feature_dropout(self.feature_norm(self.norm(feature))), **kw)
+
+    torch.manual_seed(2)
+    m, plain, x = Own(), igs_amd.GaussianSplatting2D(4, 16), torch.randn(2, 5, 16)
+    plain.load_state_dict(m.state_dict())
+    want = plain(torch.tanh(x), size=(6, 7), fused=False)
+    state = {k: v for k, v in m.__dict__.items() if k not in ("emb_scale", "feature_dropout", "dropout_seed", "_feature_norm")}
+    state["_modules"] = {k: v for k, v in m._modules.items() if k != "embedding"}
+    before = Own.__new__(Own)                            # pickled before the module had a front
+    before.__setstate__(state)
+    for c in (m, copy.deepcopy(m), before):
+        got = c(x, size=(6, 7), fused=False)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_modules_pickled_with_a_norm_and_no_flag_keep_it():
+    """State as it was when the presence of `norm` alone said that the module normalises."""
+    m, x = igs_amd.GaussianSplatting2D(4, 16, feature_norm=True), torch.randn(2, 5, 16)
+    state = {k: v for k, v in m.__dict__.items() if k != "_feature_norm"}
+    old = igs_amd.GaussianSplatting2D.__new__(igs_amd.GaussianSplatting2D)
+    old.__setstate__(state)
+    assert torch.equal(old(x, size=(6, 7), fused=False)[1], m(x, size=(6, 7), fused=False)[1])
