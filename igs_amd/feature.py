@@ -144,11 +144,12 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding
 
 def naive_embedding_lookup(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
     """Plain torch expression of `embedding_lookup` (any device, differentiable through autograd)."""
-    rows = weight[tokens]
+    V = weight.shape[0]
+    inside = (tokens >= 0) & (tokens < V)
+    rows = weight[torch.where(inside, tokens, 0)]
     if padding_idx is not None:
-        pad = (tokens == padding_idx % weight.shape[0])[..., None]
-        rows = torch.where(pad, rows.detach(), rows)
-    return rows * scale
+        rows = torch.where((tokens == padding_idx % V)[..., None], rows.detach(), rows)
+    return torch.where(inside[..., None], rows * scale, math.nan)
 
 
 # --------------------------------------------------------------------------------------

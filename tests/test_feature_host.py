@@ -354,3 +354,24 @@ def test_modules_pickled_with_a_norm_and_no_flag_keep_it():
     old = igs_amd.GaussianSplatting2D.__new__(igs_amd.GaussianSplatting2D)
     old.__setstate__(state)
     assert torch.equal(old(x, size=(6, 7), fused=False)[1], m(x, size=(6, 7), fused=False)[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32], ids=str)
+def test_plain_lookup_of_tokens_outside_the_table(dtype):
+    """The plain expression says what the operator says of them: a row of NaN, no gradient (a negative one is not taken from
+    the table's end), so that the module's debug path and the fused one agree."""
+    from oracle import feature_oracle as F
+
+    w, up = torch.randn(6, 10), torch.randn(8, 10)
+    t = torch.tensor([0, 6, -1, 5, 2 ** 31 - 1, -2 ** 31, 3, 5]).to(dtype)
+    for pad in (None, 3, -6):
+        leaf = w.clone().requires_grad_(True)
+        y = igs_amd.naive_embedding_lookup(t, leaf, 2.0, pad)
+        assert torch.equal(y.detach().nan_to_num(7.0), F.embedding(t, w, 2.0).float().nan_to_num(7.0))
+        assert y.isnan().all(-1).tolist() == [False, True, True, False, True, True, False, False]
+        (g,) = torch.autograd.grad(y, leaf, up)
+        # sums of two terms and a factor of two: exact but for one rounding of fp32
+        assert torch.allclose(g.double(), F.embedding_grad(t, up, 6, 2.0, pad)[0], rtol=2.0 ** -23, atol=0)
+    m = igs_amd.GaussianSplatting2D(4, 16, num_embeddings=11)
+    feat = m(torch.tensor([[1, -1], [11, 2]]), size=(6, 7), fused=False)[1].view(2, 2, -1)
+    assert feat.isnan().all(-1).tolist() == [[False, True], [True, False]]
