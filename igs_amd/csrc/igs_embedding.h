@@ -62,22 +62,13 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-#ifndef IGS_SORT_PER
-#define IGS_SORT_PER 8
-#endif
-constexpr int kSortPer = IGS_SORT_PER;  // keys per thread of the one-workgroup sort, at most
+constexpr int kSortPer = 8;  // keys per thread of the one-workgroup sort, at most
 constexpr int kSortOne = kSortPer * kSortThreads;
 constexpr int kSortBits = 9;     // of a digit, at most
 constexpr int kSortHeld = 4;     // keys per thread that a tile's workgroup keeps in registers
 constexpr int kSortTiles = 128;  // at most: a tile's workgroup adds up the counts of all tiles itself
-#ifndef IGS_SUM_THREADS
-#define IGS_SUM_THREADS 512
-#endif
-constexpr int kSumThreads = IGS_SUM_THREADS;
-#ifndef IGS_SUM_UNROLL
-#define IGS_SUM_UNROLL 8
-#endif
-constexpr int kUnroll = IGS_SUM_UNROLL;  // rows in a group of loads
+constexpr int kSumThreads = 512;
+constexpr int kUnroll = 8;  // rows in a group of loads
 
 template <class I>
 __device__ __forceinline__ int token_key(I t, int64_t vocab, int64_t padding) {

@@ -39,22 +39,15 @@ struct EmbedPlan {
     size_t counts_at, partial_at, bytes;  // in the workspace, behind the arrays
 };
 
-#ifndef IGS_EMBED_SUM_WAVES
-#define IGS_EMBED_SUM_WAVES 4096
-#endif
-#ifndef IGS_EMBED_SMALL
-#define IGS_EMBED_SMALL kSmall
-#endif
-#ifndef IGS_EMBED_FILL_BYTES
-#define IGS_EMBED_FILL_BYTES (64 << 10)  // per filling workgroup
-#endif
+constexpr int kSumWaves = 4096;        // of k_embed_sum on the device, about
+constexpr int kFillBytes = 64 << 10;   // per filling workgroup
 
 EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {  // n >= 1
     EmbedPlan p;
     int total = 0;  // bits of the largest key, vocab itself
     while (vocab >> total) ++total;
     const bool one = n <= kSortOne;
-    p.small = n <= IGS_EMBED_SMALL;
+    p.small = n <= kSmall;
     p.passes = (total + kSortBits - 1) / kSortBits;
     p.bits = (total + p.passes - 1) / p.passes;
     p.tiles = p.tile = 0;
@@ -71,7 +64,7 @@ EmbedPlan make_embed_plan(int64_t vocab, int D, int dtype, int64_t n) {  // n >=
     s.slices = (int)ceil_div(packs, s.lanes);
     // places per unit: short enough for so many waves on the device, eight (one group of loads) at least
     const int64_t waves = n * s.slices * s.lanes / kWave;
-    const int64_t len = ceil_div(ceil_div(waves, IGS_EMBED_SUM_WAVES), kUnroll) * kUnroll;
+    const int64_t len = ceil_div(ceil_div(waves, kSumWaves), kUnroll) * kUnroll;
     s.len = (int)(len < kUnroll ? kUnroll : len);
     const int units = (p.small ? kSortThreads : kSumThreads) / s.lanes;
     p.span = (int64_t)units * s.len;
@@ -144,7 +137,7 @@ void launch_embed_sum(const T* grad, const int* keys, const int* pos, int64_t n,
 template <class T, class I, int V>
 void launch_embed_small(const T* grad, const I* tokens, int n, int64_t vocab, int64_t padding, int D, float scale,
                         const EmbedPlan& p, T* out, hipStream_t st) {
-    const int64_t fit = IGS_EMBED_FILL_BYTES / ((int64_t)D * (int)sizeof(T));
+    const int64_t fit = kFillBytes / ((int64_t)D * (int)sizeof(T));
     const int64_t least = ceil_div(vocab, 1 << 21);  // a launch has fewer than 2^32 threads
     const int rows = (int)(fit < least ? least : at_most(fit, kSmall));
     const dim3 grid((int64_t)p.sum.groups * p.sum.slices + ceil_div(vocab, rows));
@@ -163,7 +156,7 @@ int launch_embed_bwd(const void* grad, const void* tokens, int64_t n, int64_t vo
     const int64_t total = vocab * D;
     // workgroups that fill `count` elements with zeros
     const auto filling = [](int64_t count) {
-        return at_most(ceil_div(count * (int64_t)sizeof(T), IGS_EMBED_FILL_BYTES), 1 << 20);
+        return at_most(ceil_div(count * (int64_t)sizeof(T), kFillBytes), 1 << 20);
     };
     if (n == 0) {
         hipLaunchKernelGGL((k_fill<T>), dim3(filling(total)), dim3(kSortThreads), 0, st, out, total);

@@ -51,34 +51,19 @@ NormShape norm_layout(int D, int dtype) {
 inline int norm_rows_at_once(const NormShape& s) { return s.tpr > kBlock ? 1 : kBlock / s.tpr; }
 inline int norm_elements(const NormShape& s, int dtype) { return s.one ? 1 : s.nv * (16 / dtype_bytes(dtype)); }
 
-#ifndef IGS_NORM_FWD_WGS
-#define IGS_NORM_FWD_WGS 8
-#endif
-#ifndef IGS_NORM_FWD_WGS_WIDE
-#define IGS_NORM_FWD_WGS_WIDE 2
-#endif
-#ifndef IGS_NORM_FWD_WGS_512
-#define IGS_NORM_FWD_WGS_512 1
-#endif
-#ifndef IGS_NORM_BWD_WGS
-#define IGS_NORM_BWD_WGS 4
-#endif
-#ifndef IGS_NORM_BWD_WGS_16
-#define IGS_NORM_BWD_WGS_16 2
-#endif
-#ifndef IGS_NORM_COLS_WGS
-#define IGS_NORM_COLS_WGS 4
-#endif
 // Workgroups per compute unit: each loads the weights of its columns once and, in the backward, leaves a
 // partial row of 2 D sums, so few workgroups that walk over many rows, but enough to keep the memory busy
 // (us at 2 / 4 / 6 per compute unit, backward: bf16 32768 x 1024 40 / 45 / 50, fp32 4096 x 4096
 // 46 / 57 / 69, bf16 65536 x 256 25 / 23 / 27).
+constexpr int kFwdGroups = 8, kFwdGroupsWide = 2, kFwdGroups512 = 1;  // 16 elements a thread at most; more; 512 threads
+constexpr int kBwdGroups = 4, kBwdGroups16 = 2;                       // 8 elements a thread at most; more
+constexpr int kColsGroups = 4;                                        // of k_norm_bwd_cols
 int64_t norm_fwd_groups(const NormShape& s, int64_t rows, int dtype) {
-    const int per_cu = s.tpr > kBlock ? IGS_NORM_FWD_WGS_512 : norm_elements(s, dtype) > 16 ? IGS_NORM_FWD_WGS_WIDE : IGS_NORM_FWD_WGS;
+    const int per_cu = s.tpr > kBlock ? kFwdGroups512 : norm_elements(s, dtype) > 16 ? kFwdGroupsWide : kFwdGroups;
     return at_most(ceil_div(rows, norm_rows_at_once(s)), (int64_t)device_cus() * per_cu);
 }
 int64_t norm_bwd_groups(const NormShape& s, int64_t rows, int dtype) {
-    const int per_cu = norm_elements(s, dtype) > 8 ? IGS_NORM_BWD_WGS_16 : IGS_NORM_BWD_WGS;
+    const int per_cu = norm_elements(s, dtype) > 8 ? kBwdGroups16 : kBwdGroups;
     return at_most(ceil_div(rows, norm_rows_at_once(s)), (int64_t)device_cus() * per_cu);
 }
 
@@ -91,7 +76,7 @@ int norm_plan(int64_t rows, int D, int dtype, int wdtype, igs_layer_norm_plan_t*
     int64_t P, row_sums = 0;
     if (D > kTwoPass) {  // groups of rows: two rounds of loads per wave, or as many as the device holds workgroups
         P = at_most(ceil_div(rows, 2 * kRowsAhead * (kBlock / kWave)),
-                    ceil_div((int64_t)device_cus() * IGS_NORM_COLS_WGS, norm_slices(D, dtype)));
+                    ceil_div((int64_t)device_cus() * kColsGroups, norm_slices(D, dtype)));
         row_sums = rows;
     } else {
         P = norm_bwd_groups(norm_layout(D, dtype), rows, dtype);

@@ -375,3 +375,15 @@ def test_plain_lookup_of_tokens_outside_the_table(dtype):
     m = igs_amd.GaussianSplatting2D(4, 16, num_embeddings=11)
     feat = m(torch.tensor([[1, -1], [11, 2]]), size=(6, 7), fused=False)[1].view(2, 2, -1)
     assert feat.isnan().all(-1).tolist() == [[False, True], [True, False]]
+
+
+def test_feature_kernels_have_no_build_switches():
+    """Sizes of shared arrays and the limits that keep calls within them are one constant each: nothing on a compiler's
+    command line can move a limit past its array."""
+    import os
+
+    csrc = os.path.join(os.path.dirname(feature.__file__), "csrc")
+    for name in ("igs_feature.hip", "igs_feature_common.h", "igs_feature_host.h", "igs_embedding.h", "igs_dropout.h", "igs_norm.hip",
+                 "igs_layer_norm.h"):
+        text = open(os.path.join(csrc, name)).read()
+        assert "#ifndef" not in text and "#ifdef" not in text, name
