@@ -44,15 +44,21 @@ C1_PROFILE = {
 
 def csrc_sha16():
     """First 16 hex digits of the SHA-256 over the sources of the splat's kernels, in name order: the translation
-    unit igs_gs2d.hip, the files it includes and include/igs_hip.h (other units of the library are not among them)."""
+    unit igs_gs2d.hip, the files of the tree that it includes, themselves or through others, and include/igs_hip.h
+    (other units of the library are not among them)."""
     import hashlib
     import re
 
     h = hashlib.sha256()
-    csrc = os.path.join(ROOT, "igs_amd", "csrc")
-    unit = os.path.join(csrc, "igs_gs2d.hip")
-    names = re.findall(r'^#include "(igs_\w+\.h)"', open(unit).read(), flags=re.M)
-    for path in sorted([unit] + [os.path.join(csrc, n) for n in names if n != "igs_hip.h"]) + [os.path.join(ROOT, "include", "igs_hip.h")]:
+    csrc, header = os.path.join(ROOT, "igs_amd", "csrc"), os.path.join(ROOT, "include", "igs_hip.h")
+    found, todo = set(), [os.path.join(csrc, "igs_gs2d.hip"), header]
+    while todo:
+        path = todo.pop()
+        found.add(path)
+        for name in re.findall(r'^[ \t]*#[ \t]*include[ \t]*["<]([^">]+)[">]', open(path).read(), flags=re.M):
+            near = [os.path.normpath(os.path.join(d, name)) for d in (os.path.dirname(path), csrc, os.path.dirname(header))]
+            todo += [p for p in near if os.path.isfile(p) and p not in found][:1]
+    for path in sorted(found - {header}) + [header]:
         h.update(os.path.basename(path).encode())
         h.update(open(path, "rb").read())
     return h.hexdigest()[:16]
