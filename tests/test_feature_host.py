@@ -387,3 +387,30 @@ def test_feature_kernels_have_no_build_switches():
                  "igs_layer_norm.h"):
         text = open(os.path.join(csrc, name)).read()
         assert "#ifndef" not in text and "#ifdef" not in text, name
+
+
+@pytest.mark.parametrize("n", [1025, 8192, 8193, 100000])
+def test_workspace_refusals_of_the_lookup_gradient(lib, n):
+    """More tokens than one launch takes need a workspace: one byte less than the plan's, or none at all, is refused before
+    anything is launched."""
+    p, E, big = ctypes.c_void_p(4096), _lib.EmbeddingPlan(), 1 << 40
+    for vocab, D, dtype in ((10, 8, 0), (50021, 333, 1), (1 << 20, 1024, 2)):
+        assert lib.igs_embedding_plan(vocab, D, dtype, n, ctypes.byref(E)) == 0
+        assert E.ws_bytes >= 8 * n                       # sorted keys and their places
+        for width in (4, 8):
+            bwd = lambda ws, size: lib.igs_embedding_backward(p, dtype, p, width, n, vocab, D, 1.0, -1, p, ws, size, None)
+            assert bwd(p, E.ws_bytes - 1) == -4 and bwd(p, 0) == -4
+            assert bwd(None, E.ws_bytes) == -1 and bwd(None, big) == -1
+            assert bwd(ctypes.c_void_p(4100), big) == -7
+
+
+@pytest.mark.parametrize("rows,D", [(1, 8), (10, 8), (1000, 1024), (10, 5000), (3, 100000)])
+def test_workspace_refusals_of_the_norm_gradient(lib, rows, D):
+    p, N, big = ctypes.c_void_p(4096), _lib.LayerNormPlan(), 1 << 40
+    for dtype in (0, 1, 2):
+        assert lib.igs_layer_norm_plan(rows, D, dtype, 0, ctypes.byref(N)) == 0
+        assert N.ws_bytes >= 8 * D and N.partials >= 1   # a partial row of two sums at least
+        bwd = lambda ws, size: lib.igs_layer_norm_backward(p, p, D, dtype, p, 0, p, rows, D, 0, 0, None, 0, p, p, p, ws, size, None)
+        assert bwd(p, N.ws_bytes - 1) == -4 and bwd(p, 0) == -4
+        assert bwd(None, N.ws_bytes) == -1 and bwd(None, big) == -1
+        assert bwd(ctypes.c_void_p(4104), big) == -7

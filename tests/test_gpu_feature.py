@@ -853,3 +853,139 @@ def test_lazily_negated_tensors(igs, dev):
         assert g.is_neg() and torch.equal(*[torch.autograd.grad(y, leaf, v, retain_graph=True)[0] for v in (g, g.resolve_neg())])
     with pytest.raises(RuntimeError, match="seed"):
         igs.dropout(x, 0.3, neg(torch.tensor([5], device=dev)))
+
+
+# ---------------------------------------------------------------------------------- tensors past the caches
+def check_here(got, ref, tol, what):
+    """`check` without the copy to the host."""
+    assert got.shape == ref.shape, what
+    err = (got.detach().to(F64) - ref).abs()
+    assert bool((err <= tol).all()), (what, float((err / tol).max()))
+
+
+def big_normal(shape, seed, dtype, dev, shift, mean=0.0, std=1.0):
+    """Normal numbers made on the device, `shift` elements behind an aligned address."""
+    g = torch.Generator(dev).manual_seed(seed)
+    n = math.prod(shape)
+    flat = torch.empty(n + shift, device=dev, dtype=dtype)
+    flat[shift:] = (torch.randn(n, generator=g, device=dev) * std + mean).to(dtype)
+    return flat[shift:].view(shape)
+
+
+# (rows, D): rows that are and are not whole packs, narrow ones, ones of more than 4096 elements, ones shorter than a pack;
+# 192 MB or more each, from which on tensors go past the caches
+PAST_CACHES = [(torch.bfloat16, torch.float32, 98611, 1021, 0), (torch.float32, torch.float32, 49311, 1021, 1),
+               (torch.float16, torch.float16, 98611, 1021, 3), (torch.float32, torch.float32, 49157, 1024, 0),
+               (torch.bfloat16, torch.bfloat16, 4194307, 25, 1), (torch.float16, torch.float32, 24571, 4101, 0),
+               (torch.float32, torch.float32, 6133, 8207, 1), (torch.float32, torch.float32, 16777219, 3, 0)]
+
+
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("dtype,wdtype,R,D,shift", PAST_CACHES, ids=str)
+def test_norm_past_the_caches(igs, dev, dtype, wdtype, R, D, shift, p):
+    """Every value of the forward that a backward follows, of the forward alone and of the three gradients against the
+    64-bit definition, by the bounds of the other sizes; the two forwards bit for bit."""
+    assert R * D * dtype.itemsize >= 192 << 20
+    x, up = big_normal((R, D), 1, dtype, dev, shift, 0.4, 1.7), big_normal((R, D), 2, dtype, dev, shift)
+    assert shift == 0 or x.data_ptr() % 16
+    w, b = normal((D,), 3, wdtype, 1.0, 0.3).to(dev), normal((D,), 4, wdtype).to(dev)
+    factors = None
+    if p:
+        t = round(p * 65536)
+        factors = igs.dropout_keep_mask((R, D), p, 11, 3, dev).to(F64) * (65536 / (65536 - t))
+    kw = dict(dropout_p=p, seed=11, offset=3) if p else {}
+    lv = [v.requires_grad_(True) for v in (x, w, b)]
+    y = igs.layer_norm(*lv, **kw)
+    with torch.no_grad():
+        assert torch.equal(igs.layer_norm(*lv, **kw), y)
+    grads = torch.autograd.grad(y, lv, up)
+    x, w, b = [v.detach() for v in lv]
+    ref = F.layer_norm(x, w, b, 1e-5, factors)[0]
+    check_here(y, ref, norm_tolerance(x, w, b, 1e-5, factors, ref, dtype), "y")
+    refs = F.layer_norm_grad(up, x, w, 1e-5, factors)
+    tols = norm_grad_tolerances(up, x, w, 1e-5, factors, refs, (dtype, wdtype))
+    for name, got, r, tol in zip(("dx", "dw", "db"), grads, refs, tols):
+        check_here(got, r, tol, name)
+
+
+@pytest.mark.parametrize("dtype,n,D,shift", [(torch.bfloat16, 98611, 1021, 1), (torch.float32, 49311, 1021, 1), (torch.float16, 98611, 1021, 0),
+                                             (torch.float32, 16777219, 3, 0), (torch.bfloat16, 4194307, 25, 3)], ids=str)
+def test_lookup_past_the_caches(igs, dev, dtype, n, D, shift):
+    """Rows of a misaligned table, some tokens outside it, come bit for bit; the gradient of a misaligned upstream of whole
+    numbers, whose sums are exact in any order, does too."""
+    assert n * D * dtype.itemsize >= 192 << 20
+    V = 7001
+    w = big_normal((V, D), 1, dtype, dev, shift).requires_grad_(True)
+    g = torch.Generator(dev).manual_seed(2)
+    t = torch.randint(0, V, (n,), generator=g, device=dev)
+    t[::1000], t[1::1000] = -1, V
+    t[5::7] = 13                                             # a frequent one: an exact sum of 2^23 ones at most
+    inside = (t >= 0) & (t < V)
+    y = igs.embedding_lookup(t, w)
+    assert torch.equal(y[inside], w.detach()[t[inside]]) and bool(y[~inside].isnan().all())
+    flat = torch.empty(n * D + shift, device=dev, dtype=dtype)
+    flat[shift:] = torch.randint(-1, 2, (n * D,), generator=g, device=dev, dtype=torch.int8).to(dtype)
+    up = flat[shift:].view(n, D)
+    (got,) = torch.autograd.grad(y, w, up)
+    want = torch.zeros(V, D, device=dev).index_add_(0, t[inside], up[inside].float())
+    assert torch.equal(got, want.to(dtype))
+
+
+# ---------------------------------------------------------------------------------- bit equality of views and of the module
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_views_give_the_bits_of_their_copies(igs, dev, dtype):
+    """The arrangement of a row over threads is a function of its length and type alone, whatever its address and stride."""
+    base, flat = normal((6, 10, 48), 1, dtype).to(dev), normal((6 * 48 + 5,), 2, dtype).to(dev)
+    views = (base[..., :40], base[:, ::2], base[..., 3:36], base.transpose(0, 1), base[..., ::2], flat[1:289].view(6, 48), flat[5:].view(6, 48),
+             flat[3:261].view(2, 129), base[:1].expand(4, 10, 48), base[:, :1].expand(6, 3, 48), base[2, 3], base[..., 7:8], base[:, :0])
+    for v in views:
+        D = v.shape[-1]
+        w, b = normal((D + 1,), 3, dtype, 1.0, 0.3).to(dev)[1:], normal((D,), 4, dtype).to(dev)
+        up = normal(tuple(v.shape), 5, dtype).to(dev)
+        res = []
+        for x in (v, v.clone(memory_format=torch.contiguous_format)):
+            x = x.detach().requires_grad_(True)
+            ws = [w.detach().requires_grad_(True), b.detach().requires_grad_(True)]
+            y = igs.layer_norm(x, *ws, dropout_p=0.2, seed=5)
+            res.append((y, *torch.autograd.grad(y, [x, *ws], up)))
+        for a, c in zip(*res):
+            assert a.shape == c.shape and torch.equal(a, c)
+
+
+def test_module_is_its_operators_and_the_plain_module(igs, dev):
+    """The module with its front against the operators called one by one in front of the module without: image, features and
+    every gradient bit for bit (the same kernels on the same numbers)."""
+    torch.manual_seed(1)
+    m = igs.GaussianSplatting2D(8, 128, num_embeddings=50, emb_scale=1.5, padding_idx=0, feature_norm=True, feature_dropout=0.2).to(dev)
+    m.dropout_seed = 1234
+    plain = igs.GaussianSplatting2D(8, 128).to(dev)
+    plain.load_state_dict({k: v for k, v in m.state_dict().items() if k.startswith("proj")})
+    t, up = torch.randint(0, 50, (2, 24), device=dev), torch.randn(2, 3, 20, 28, device=dev)
+    img, feat = m(t, size=(20, 28))
+    img.backward(up)
+    lv = [v.detach().clone().requires_grad_(True) for v in (m.embedding.weight, m.norm.weight, m.norm.bias)]
+    f = igs.layer_norm(igs.embedding_lookup(t, lv[0], 1.5, 0), lv[1], lv[2], m.norm.eps, 0.2, 1234)
+    want, want_feat = plain(f, size=(20, 28))
+    want.backward(up)
+    assert torch.equal(img, want) and torch.equal(feat, want_feat)
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip((m.embedding.weight, m.norm.weight, m.norm.bias, *m.proj.parameters()),
+                                                           (*lv, *plain.proj.parameters())))
+    assert bool(m.embedding.weight.grad.any()) and not m.embedding.weight.grad[0].any()
+
+
+def test_direct_calls_that_would_read_beside_a_tensor_are_refused(igs, dev):
+    """The registered operators with what the public functions never pass: refused on the host."""
+    ops = torch.ops.igs_amd
+    x, stats = torch.randn(3, 16, device=dev).bfloat16(), torch.zeros(3, 2, device=dev)
+    for wtype in (torch.int8, torch.uint8, torch.float64, torch.float16):
+        w = torch.ones(16, device=dev, dtype=wtype)
+        for weight, bias in ((w, None), (None, w), (w, w)):
+            with pytest.raises(RuntimeError):
+                ops.layer_norm_fwd(x, weight, bias, 1e-5, 0, 0, None, 0)
+            with pytest.raises(RuntimeError):
+                ops.layer_norm_bwd(x, x, weight, bias, stats, 0, 0, None, 0)
+    for threshold in (2 ** 32, -1, 65537):
+        for call in (lambda: ops.dropout(x, threshold, 0, None, 0), lambda: ops.layer_norm_fwd(x, None, None, 1e-5, threshold, 0, None, 0),
+                     lambda: ops.layer_norm_bwd(x, x, None, None, stats, threshold, 0, None, 0)):
+            with pytest.raises(RuntimeError, match="threshold"):
+                call()
