@@ -1,4 +1,4 @@
-"""`torch.library` registration of the HIP splat, for callers under `torch.compile`.
+"""`torch.library` registration of the HIP splat, for callers under `torch.compile` and dispatch modes (make_fx).
 
 The reference wraps `render` in `torch.compile(dynamic=True)` (src/igs/gs2d.py:525) and its users
 compile whole models around it.  ctypes calls are opaque to Dynamo, so the splat is registered as

@@ -418,6 +418,13 @@ def problem_dims(kind: int, params: Sequence[Tensor]):
     raise ValueError(f"unknown parameterisation {kind}")
 
 
+def recorded() -> bool:
+    """Whether the registered operators are to be called: under torch.compile and torch.export, and under a dispatch mode
+    (make_fx and the like), which of an eager call sees the allocations and not what the library writes.  (torch.jit.trace
+    records an autograd.Function as a node.)"""
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+
+
 def require_gpu(t: Tensor):
     if t.device.type != "cuda":
         raise RuntimeError("the fused Gaussian-splatting path runs on the GPU only (HIP kernels); got a tensor on "

@@ -20,7 +20,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _lib, _ops, feature as _feature
-from ._splat import KIND_COVINV, KIND_FEATURE, KIND_SCALE_ROT, channel_groups, run_backward, run_forward
+from ._splat import KIND_COVINV, KIND_FEATURE, KIND_SCALE_ROT, channel_groups, recorded, run_backward, run_forward
 
 Tensor = torch.Tensor
 
@@ -106,7 +106,7 @@ class GaussianSplatting2DKernel:
 
     A plain class with the `torch.autograd.Function` calling convention rather than a Function
     itself: `.apply` routes eager callers to the autograd.Function above and callers under
-    `torch.compile` to the registered operators (Dynamo would otherwise trace into the ctypes
+    `torch.compile`, `make_fx` and the like to the registered operators (Dynamo would otherwise trace into the ctypes
     calls of a Function's forward).
     """
 
@@ -126,7 +126,7 @@ class GaussianSplatting2DKernel:
             return torch.cat([GaussianSplatting2DKernel.apply(x, y, position, cov_inv_00, cov_inv_01, cov_inv_11,
                                                               alphas, colors[..., lo:hi], eps)
                               for lo, hi in channel_groups(C)], dim=1)
-        if torch.compiler.is_compiling():
+        if recorded():
             B, N = position.shape[:2]
             params = [position, cov_inv_00.reshape(B, N), cov_inv_01.reshape(B, N), cov_inv_11.reshape(B, N),
                       alphas, colors]
@@ -212,7 +212,7 @@ def _render_fused(positions, colors, scales, rotations, alphas, x_grid, y_grid, 
                         positions.shape[1], colors.shape[-1], positions.dtype)
     if empty is not None:
         return empty
-    if torch.compiler.is_compiling():
+    if recorded():
         return _ops.splat(KIND_SCALE_ROT, [positions, colors, scales, rotations, alphas], x_grid, y_grid, eps,
                           colors.shape[-1], positions.dtype)
     return _RenderFused.apply(positions, colors, scales, rotations, alphas, x_grid, y_grid, eps)
@@ -223,7 +223,7 @@ def _render_from_feature(gs_feature, pos_offset, x_grid, y_grid, eps):
                         gs_feature.shape[0], gs_feature.shape[1], gs_feature.shape[-1] - 6, gs_feature.dtype)
     if empty is not None:
         return empty
-    if torch.compiler.is_compiling():
+    if recorded():
         params = [gs_feature] if pos_offset is None else [gs_feature, pos_offset]
         return _ops.splat(KIND_FEATURE, params, x_grid, y_grid, eps, gs_feature.shape[-1] - 6, gs_feature.dtype)
     return _RenderFromFeature.apply(gs_feature, pos_offset, x_grid, y_grid, eps)

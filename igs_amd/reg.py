@@ -4,7 +4,7 @@ loss = mean over the B*N rows of relu(max_{j != i} cos(x_i, x_j) + 1).  The refe
 whole [B, N, N] similarity matrix (bmm, diagonal fill, row max) under `torch.compile`; here the
 row maxima come out of a tiled kernel that never stores the matrix, and the backward sends the
 gradient through each row's nearest neighbour only, as autograd does for `max`.  Eager callers go
-through a `torch.autograd.Function`; under `torch.compile` the same two library calls are the
+through a `torch.autograd.Function`; under `torch.compile` and dispatch modes the same two library calls are the
 registered operators `igs_amd::koleo_fwd` / `igs_amd::koleo_bwd`.  There is no CPU path: tensors
 must live on the GPU.
 """
@@ -15,7 +15,7 @@ from typing import List
 import torch
 
 from . import _lib
-from ._splat import _ptr, _stream, require_gpu
+from ._splat import _ptr, _stream, recorded, require_gpu
 
 Tensor = torch.Tensor
 
@@ -145,7 +145,7 @@ def koleo_diversity_loss(features: Tensor) -> Tensor:
         # vectors normalise to zero, every similarity is 0, loss 1)
         return (features.sum() * 0 + (float("nan") if B == 0 else 1.0)).to(features.dtype)
     x = features.to(torch.float32).contiguous()
-    if torch.compiler.is_compiling():
+    if recorded():
         loss = torch.ops.igs_amd.koleo_fwd(x)[0]
     else:
         loss = _Koleo.apply(x)

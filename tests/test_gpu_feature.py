@@ -989,3 +989,38 @@ def test_direct_calls_that_would_read_beside_a_tensor_are_refused(igs, dev):
                      lambda: ops.layer_norm_bwd(x, x, None, None, stats, threshold, 0, None, 0)):
             with pytest.raises(RuntimeError, match="threshold"):
                 call()
+
+
+class Front(torch.nn.Module):
+    """Tokens -> (image, Gaussians, diversity loss of the normalised tokens) through the module and what stands around it."""
+
+    def __init__(self, igs, dev, size):
+        super().__init__()
+        self.size = size
+        torch.manual_seed(1)
+        self.m = igs.GaussianSplatting2D(4, 32, num_embeddings=30, emb_scale=1.5, feature_norm=True).to(dev)
+        self.koleo = igs.koleo_diversity_loss
+
+    def forward(self, t):
+        img, feat = self.m(t, size=self.size)
+        return img, feat, self.koleo(self.m.embedding.weight[None])
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("how", ["jit", "fx"])
+def test_traced_module_from_tokens_to_the_image(igs, dev, how, grad):
+    """A trace of the whole module, its first use at this image size, computes the image for other tokens; the module itself
+    works afterwards."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f = Front(igs, dev, (9, 11 + 2 * ["jit", "fx"].index(how) + grad))
+    a, b = [torch.randint(0, 30, (2, 6), device=dev, generator=torch.Generator(dev).manual_seed(k)) for k in (1, 2)]
+    with torch.set_grad_enabled(grad):
+        if how == "jit":
+            traced = torch.jit.trace(f, (a,), check_trace=False)
+        else:
+            traced = make_fx(f)(a)
+    want, other = f(b), f(a)
+    assert bool(want[0].isfinite().all()) and not torch.equal(want[0], other[0])
+    for x, y in zip(traced(b), want):
+        assert torch.equal(x, y)
