@@ -243,16 +243,24 @@ def _cov_inverse_torch(scales, rotations, eps):
     return inv[..., 0, 0, None, None], inv[..., 0, 1, None, None], inv[..., 1, 1, None, None]
 
 
-@functools.lru_cache(maxsize=32)
-def _grid_vectors(h: int, w: int, device):
-    """The two coordinate vectors of xy_grid, kept per (size, device) for the module's forward.
-    Built outside inference mode so that a first call under torch.inference_mode() does not leave
-    inference tensors behind for later training calls."""
+def _new_grid_vectors(h: int, w: int, device):
+    """The two coordinate vectors of xy_grid."""
     aspect_ratio = h / w
     h_range = aspect_ratio ** 0.5
     w_range = 1 / aspect_ratio ** 0.5
     with torch.inference_mode(False):
         return torch.linspace(-w_range, w_range, w).to(device), torch.linspace(-h_range, h_range, h).to(device)
+
+
+# Kept per (size, device) for the module's forward.  Built outside inference mode so that a first call under
+# torch.inference_mode() does not leave inference tensors behind for later training calls.
+_kept_grid_vectors = functools.lru_cache(maxsize=32)(_new_grid_vectors)
+
+
+def _grid_vectors(h: int, w: int, device):
+    """The kept vectors; new ones where the operators are recorded (torch.export traces with fake tensors, which a later
+    eager call could not use)."""
+    return (_new_grid_vectors if recorded() else _kept_grid_vectors)(h, w, device)
 
 
 class GaussianSplatting2D(nn.Module):

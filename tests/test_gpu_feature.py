@@ -1007,19 +1007,21 @@ class Front(torch.nn.Module):
 
 
 @pytest.mark.parametrize("grad", [False, True])
-@pytest.mark.parametrize("how", ["jit", "fx"])
+@pytest.mark.parametrize("how", ["jit", "fx", "export"])
 def test_traced_module_from_tokens_to_the_image(igs, dev, how, grad):
     """A trace of the whole module, its first use at this image size, computes the image for other tokens; the module itself
     works afterwards."""
     from torch.fx.experimental.proxy_tensor import make_fx
 
-    f = Front(igs, dev, (9, 11 + 2 * ["jit", "fx"].index(how) + grad))
+    f = Front(igs, dev, (9, 11 + 2 * ["jit", "fx", "export"].index(how) + grad))
     a, b = [torch.randint(0, 30, (2, 6), device=dev, generator=torch.Generator(dev).manual_seed(k)) for k in (1, 2)]
     with torch.set_grad_enabled(grad):
         if how == "jit":
             traced = torch.jit.trace(f, (a,), check_trace=False)
-        else:
+        elif how == "fx":
             traced = make_fx(f)(a)
+        else:
+            traced = torch.export.export(f, (a,), strict=False).module()
     want, other = f(b), f(a)
     assert bool(want[0].isfinite().all()) and not torch.equal(want[0], other[0])
     for x, y in zip(traced(b), want):
