@@ -1026,3 +1026,37 @@ def test_traced_module_from_tokens_to_the_image(igs, dev, how, grad):
     assert bool(want[0].isfinite().all()) and not torch.equal(want[0], other[0])
     for x, y in zip(traced(b), want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_registered_operators_by_opcheck_and_with_dynamic_sizes(igs, dev, dtype):
+    """torch's own checks of the five operators (schema, autograd registration, fake tensors, AOT dispatch with static and
+    dynamic sizes), and the chain compiled for changing sizes against the eager one, forward and backward."""
+    ops, check = torch.ops.igs_amd, torch.library.opcheck
+    t, seed = torch.randint(0, 9, (2, 5), device=dev), torch.tensor([5], device=dev)
+    w, x = torch.randn(9, 16, device=dev).to(dtype).requires_grad_(), torch.randn(2, 5, 16, device=dev).to(dtype).requires_grad_()
+    lw, lb = torch.randn(16, device=dev, requires_grad=True), torch.randn(16, device=dev, requires_grad=True)
+    d = lambda v: v.detach()
+    stats = ops.layer_norm_fwd(d(x), d(lw), None, 1e-5, 0, 0, None, 0)[1]
+    turned = d(x).transpose(0, 1).requires_grad_()
+    for op, args in ((ops.embedding_fwd, (t, w, 2.0, -1)), (ops.embedding_bwd, (d(x), t, 9, 2.0, 3)), (ops.layer_norm_fwd, (x, lw, lb, 1e-5, 100, 7, None, 0)),
+                     (ops.layer_norm_fwd, (turned, lw, None, 1e-5, 100, 7, seed, 0)), (ops.layer_norm_bwd, (d(x), d(x), d(lw), d(lb), stats, 100, 7, None, 0)),
+                     (ops.dropout, (x, 30000, 7, seed, 3)), (ops.dropout, (turned, 30000, 7, None, 3))):
+        check(op.default, args)
+
+    def fn(t, w, a, b, seed):
+        f = igs.layer_norm(igs.embedding_lookup(t, w, 1.5, -1), a, b, dropout_p=0.3, seed=seed, offset=2)
+        return igs.dropout(f, 0.2, seed, 9)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(fn, fullgraph=True, dynamic=True)
+    for n, D in ((7, 24), (130, 33), (1, 40)):
+        leaves = [torch.randn(9, D, device=dev).to(dtype), torch.randn(D, device=dev), torch.randn(D, device=dev).to(dtype)]
+        tokens, s, up = torch.randint(0, 9, (n,), device=dev), torch.tensor([n], device=dev), torch.randn(n, D, device=dev).to(dtype)
+        res = []
+        for f in (fn, compiled):
+            lv = [v.detach().requires_grad_(True) for v in leaves]
+            y = f(tokens, *lv, s)
+            res.append((y.detach(), *torch.autograd.grad(y, lv, up)))
+        for a, c in zip(*res):
+            assert torch.equal(a, c)
