@@ -56,6 +56,11 @@ __global__ __launch_bounds__(kBlock) void k_embed_fwd(const T* __restrict__ weig
 //                               partial rows
 //   k_embed_join                adds those
 //   k_embed_small               all of it, for few tokens
+// us of the whole gradient at the borders, this side / the other (a table of 8192 rows, uniform tokens, device time):
+//   kSmall    one launch / three   1024 tokens: fp32 x 64 12.9 / 14.6, fp16 x 333 12.2 / 13.6, fp32 x 1024 13.0 / 16.3;
+//                                  513: 10.0 / 12.7, 11.7 / 13.4, 12.6 / 15.4; one token in all 1024 places 25.6 / 16.8
+//   kSortOne  one workgroup / tiles   8192 tokens: 24.7 / 25.5, 25.4 / 26.3, 34.6 / 35.7; 4097: 20.1 / 25.2, 20.6 / 25.7,
+//                                  25.9 / 30.6; and 8193, in tiles: fp16 x 333 26.1, fp32 x 1024 35.9
 // The sort waits on memory and keeps few compute units busy; the other workgroups of its launches fill the
 // table's gradient with zeros meanwhile, so that k_embed_sum writes the rows that tokens name and no more.
 // Every sum has a fixed order; the atomics are integer counters in LDS.
@@ -486,11 +491,10 @@ __device__ __forceinline__ int run_border(const int* keys, int n, int at) {
 }
 
 // Few tokens (up to kSmall): the whole gradient in one launch and without a workspace, a small step being bound by its
-// launches (1024 tokens of 8192 x 1024 in fp32, training step: 47 us, 53 in three launches).  Workgroup (group, slice)
+// launches (1024 tokens of 8192 x 1024 in fp32: 13 us, 16 in three launches).  Workgroup (group, slice)
 // sorts all tokens for itself and adds up the runs that begin in its group's places; the workgroups behind those
 // each look all tokens up for `zero_rows` rows of the table and write zeros into the rows that none names.  A run is not
-// shared among workgroups here: one token in all 1024 places takes 32 us (uniform ones 17, as in three launches), which
-// bounds kSmall.
+// shared among workgroups here: one token in all 1024 places takes 26 us (17 in three launches), which bounds kSmall.
 constexpr int kSmall = kSortThreads;
 template <class T, class I, int V, bool kWide>
 __global__ __launch_bounds__(kSortThreads) void k_embed_small(const T* __restrict__ grad, const I* __restrict__ tokens,

@@ -117,7 +117,8 @@ __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
 
 // Philox4x32, seven rounds (Salmon, Moraes, Dror, Shaw 2011: the fewest that pass their test batteries;
 // dropout asks no more of its numbers).  128 bits per block serve eight elements with 16 bits each,
-// which keeps the integer products (quarter rate) below the time of the memory traffic.
+// which keeps the integer products (quarter rate) below the time of the memory traffic.  A pack of eight 16-bit elements
+// takes one block; a pack of four fp32 ones takes one too and uses half of it, so that fp32 computes each block twice.
 __device__ __forceinline__ void philox(uint64_t block, const PhiloxKey& key, uint32_t (&w)[4]) {
     uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = key.o0, c3 = key.o1;
     uint32_t k0 = key.k0, k1 = key.k1;

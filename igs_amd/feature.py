@@ -271,7 +271,8 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0) -> Tensor:
     forward and again in the backward, and never stored.  seed: an int in [0, 2^63), or an int64 tensor of
     one element on the device, read when the kernel runs: change it between replays of a captured graph
     (and not between a forward and its backward).  Calls of one step that must differ take different
-    offsets.  A dropped element is 0 also where x is NaN or infinite."""
+    offsets.  A dropped element is 0 also where x is NaN or infinite.  Where nothing can be dropped
+    (p < 2^-17) the result is x itself, as with torch's dropout, and not a copy."""
     threshold = dropout_threshold(p)
     if threshold == 0:
         return x
